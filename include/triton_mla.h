@@ -492,6 +492,50 @@ int tmla_mla_project(const void* x, int64_t x_stride, const void* w, int64_t w_s
                      int32_t n, int32_t k, int32_t dtype, void* y, int64_t y_stride, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/*
+ * Decode over shared prefixes: tmla_mla_decode of a paged cache for a batch
+ * whose sequences, in groups of consecutive ones, begin with the same pages.
+ * Group g is the sequences [group_starts[g], group_starts[g + 1]); its rows
+ * attend to the group's prefix once, 128 rows (query tokens x heads x
+ * sequences) to a workgroup, and every sequence to its own tokens behind it;
+ * a log-sum-exp merge joins the two. No counterpart in the reference, whose
+ * kernels read each sequence's cache on their own (kernel.py:83-123).
+ *
+ *   q, out, lse   as tmla_mla_decode_causal takes them: q_len * num_heads rows
+ *                 a sequence, query token t of row t * num_heads + h; out and
+ *                 q with element strides (stride_b, stride_h, 1). lse may be
+ *                 NULL.
+ *   prefix_lens   [num_groups] tokens that each group shares, or NULL:
+ *                 prefix_len for every group. Of these, whole 64-token tiles
+ *                 are shared, no more than the group's shortest sequence
+ *                 holds before its query tokens (sequences of length <= 0
+ *                 aside); they are read through the block-table row of the
+ *                 group's first sequence of positive length.
+ *   group_starts  [num_groups + 1], ascending, or NULL: one group of the
+ *                 whole batch (num_groups 1). Bounds out of order or outside
+ *                 [0, batch] leave groups shorter or empty; sequences outside
+ *                 every group share nothing.
+ *   num_workers   workgroups that share the work (the compute units), at most
+ *                 65535.
+ *   workspace     tmla_shared_workspace_bytes(batch, q_len * num_heads,
+ *                 num_groups, num_workers) bytes, 16-byte aligned, no
+ *                 initialisation (0 bytes: a call too large for it).
+ *
+ * Lengths past the block table (bt_cols * page_size tokens) are cut to it.
+ * num_groups at most 4096; head_dim_v 512 and rope_dim 64 in bf16 or fp16.
+ * Three launches, no host synchronisation; the same inputs give the same bits.
+ */
+size_t tmla_shared_workspace_bytes(int32_t batch, int32_t num_heads, int32_t num_groups, int32_t num_workers);
+int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* kv,
+                           int64_t kv_stride_0, int64_t kv_stride_1, int64_t num_blocks,
+                           int32_t page_size, const int32_t* block_table, int64_t bt_stride_b,
+                           int32_t bt_cols, const int32_t* cache_seqlens, const int32_t* prefix_lens,
+                           int32_t prefix_len, const int32_t* group_starts, int32_t num_groups,
+                           int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim_v,
+                           int32_t rope_dim, int32_t dtype, float softmax_scale, int32_t num_workers,
+                           void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,32 @@ constexpr float kNoMax = -__FLT_MAX__;  // running max of a head that has seen n
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Work of a decode over shared prefixes: up to 128 query rows (one query
+// token's head of one sequence each, in the order sequence, token, head)
+// against a run of 64-token tiles that all of them read through the block
+// table's row `seq`: the prefix of a group of sequences, or what one sequence
+// has of its own behind it. On the line that the workers share (as the
+// balanced partition's straddling ranges do) the item's first tile is at
+// `pos`, after kSegCostTiles extra positions. Its pieces' partial rows lie one
+// after another, `rows` each, from mid_row on.
+struct SharedItem {
+  int32_t row0, rows;
+  int32_t seq;
+  int32_t tile0, tiles;   // tiles 0: nothing to do (and no positions)
+  int32_t len;            // tokens of `seq` that the item's tiles may hold
+  int32_t causal;         // whether a row's query token hides tokens at the end
+  int32_t pos;
+  int32_t first_worker, pieces;
+  int32_t mid_row;
+  int32_t pad[5];
+};
+static_assert(sizeof(SharedItem) == 64, "one cache line's half per item");
+struct SharedHeader {
+  int32_t items, prefix_items;  // prefixes first, then the sequences' own tokens
+  int32_t chunk, total;         // positions per worker, and in all
+};
+constexpr int kSharedRows = 128;
+
 struct PartialArgs {
   const char* q;           // element pointer (bytes)
   int64_t q_sb, q_sh;      // element strides
@@ -58,6 +84,16 @@ struct PartialArgs {
   // sc_s0 + row_in_page * sc_s1] (dense caches: sequence instead of page)
   const float* kv_scale;
   int64_t sc_s0, sc_s1;    // element strides
+};
+
+// Shared prefixes: the work items and where each worker's range of them
+// begins, as the plan kernel of mla_decode_shared.hip wrote them. num_heads is
+// the rows of a sequence (query tokens x heads). A type of its own: the other
+// kernels' arguments, and so their code, stay as they are.
+struct SharedArgs : PartialArgs {
+  const SharedHeader* header;
+  const SharedItem* items;
+  const int32_t* worker_item;
 };
 
 // ---------------------------------------------------------------------------
@@ -430,5 +466,9 @@ hipError_t launch_partial_fp8(const PartialArgs& a, dim3 grid, int dtype, bool p
 // Stage 1 over a 16-bit cache with at most 16 heads per workgroup
 // (mla_decode_g16.hip): grid = (workers, head groups of 16).
 hipError_t launch_partial_g16(const PartialArgs& a, dim3 grid, int dtype, bool paged, hipStream_t stream);
+
+// Stage 1 over shared prefixes (mla_decode.hip): grid = workers; uni: pages
+// of a power of two of whole 32-token sub-tiles.
+hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, hipStream_t stream);
 
 }  // namespace tmla

@@ -352,4 +352,83 @@ inline int check_generic(const GenericCall& c, const void* workspace, size_t ws_
   return TMLA_OK;
 }
 
+// ---------------------------------------------------------------------------
+// Decode over shared prefixes (mla_decode_shared.hip)
+// ---------------------------------------------------------------------------
+constexpr int kSharedMaxGroups = 4096;  // what the plan kernel's LDS holds
+constexpr int kSharedMaxWorkers = 65535;
+constexpr int32_t kSharedItemBytes = 64;
+
+struct SharedCall {
+  int32_t batch, q_len, heads, groups, workers, dv, dr, dtype, page_size, bt_cols;
+  int64_t num_blocks, kv_stride_1;
+};
+
+// Work items of a call: the groups' prefixes in blocks of 128 rows (a group's
+// last one may be shorter; no more groups that hold a sequence than
+// sequences), and each sequence's own tokens in blocks of 128 of its rows.
+inline int64_t shared_prefix_items(int64_t batch, int64_t rows, int64_t groups) {
+  return batch * rows / 128 + (groups < batch ? groups : batch);
+}
+inline int64_t shared_own_items(int64_t batch, int64_t rows) { return batch * ((rows + 127) / 128); }
+
+// Workspace: the plan kernel's output, then the partials' lse values and the
+// partials (512 values of 16 bits a row). Every piece of an item has the
+// item's rows; there are at most workers + items pieces, those of a
+// sequence's own tokens of at most min(rows, 128) rows.
+struct SharedWs {
+  size_t items, worker_item, seq_info, mid_lse, mid_o;
+  size_t total;  // 0: invalid or too large
+};
+inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t workers) {
+  SharedWs w{0, 0, 0, 0, 0, 0};
+  if (batch < 0 || rows <= 0 || groups <= 0 || workers <= 0) return w;
+  if ((int64_t)batch * rows > INT32_MAX / 2) return w;
+  const int64_t np = shared_prefix_items(batch, rows, groups), ns = shared_own_items(batch, rows);
+  const int64_t mid = (workers + np) * 128 + ns * (rows < 128 ? rows : 128);
+  if (mid > INT32_MAX) return w;  // row numbers are 32 bits
+  auto al = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  w.items = 256;
+  w.worker_item = w.items + (size_t)al((np + ns) * kSharedItemBytes);
+  w.seq_info = w.worker_item + (size_t)al((int64_t)workers * 4);
+  w.mid_lse = w.seq_info + (size_t)al((int64_t)batch * 8);
+  w.mid_o = w.mid_lse + (size_t)al(mid * 4);
+  w.total = w.mid_o + (size_t)(mid * 1024);
+  return w;
+}
+
+// Tokens the block table can name; lengths are cut to it (and kept below
+// 2^31 with the sub-tiles that are looked ahead to).
+inline int32_t shared_capacity(const SharedCall& c) {
+  const int64_t cap = (int64_t)c.bt_cols * c.page_size;
+  return (int32_t)(cap < INT32_MAX - 256 ? cap : INT32_MAX - 256);
+}
+
+inline int check_shared(const SharedCall& c, const void* workspace, size_t ws_bytes) {
+  if (c.batch < 0 || c.heads <= 0 || c.q_len < 1)
+    return fail(TMLA_ERR_INVALID_ARGUMENT, "batch must be >= 0, num_heads and q_len > 0");
+  if (c.dtype != TMLA_BF16 && c.dtype != TMLA_FP16) return fail(TMLA_ERR_INVALID_ARGUMENT, "dtype must be TMLA_BF16 or TMLA_FP16");
+  if (c.dv != 512 || c.dr != 64) return fail(TMLA_ERR_UNSUPPORTED, "head_dim_v must be 512 and rope_dim 64");
+  if (c.groups < 1) return fail(TMLA_ERR_INVALID_ARGUMENT, "num_groups must be >= 1");
+  if (c.groups > kSharedMaxGroups) return fail(TMLA_ERR_UNSUPPORTED, "num_groups must be at most 4096");
+  if (c.workers < 1 || c.workers > kSharedMaxWorkers)
+    return fail(TMLA_ERR_INVALID_ARGUMENT, "num_workers must be in [1, 65535]");
+  if (c.batch == 0) return TMLA_OK;
+  if (c.page_size <= 0 || c.num_blocks <= 0 || c.bt_cols <= 0)
+    return fail(TMLA_ERR_INVALID_ARGUMENT, "page_size, num_blocks and bt_cols must be > 0");
+  if (c.kv_stride_1 <= 0 || c.kv_stride_1 > (1 << 25))
+    return fail(TMLA_ERR_UNSUPPORTED, "kv token stride must be in (0, 2^25] elements");
+  const int64_t rows = (int64_t)c.q_len * c.heads;
+  if (rows > 65535 * 4) return fail(TMLA_ERR_UNSUPPORTED, "q_len * num_heads must be at most 262140");
+  const size_t need = shared_ws(c.batch, (int32_t)rows, c.groups, c.workers).total;
+  // the line's positions are 32 bits
+  const int64_t items = shared_prefix_items(c.batch, rows, c.groups) + shared_own_items(c.batch, rows);
+  const int64_t tiles = (int64_t)shared_capacity(c) / kTileTokens + 1 + kSegCostTiles;
+  if (need == 0 || items * tiles > INT32_MAX - 2 * kSharedMaxWorkers)
+    return fail(TMLA_ERR_UNSUPPORTED, "batch, heads and block-table width are too large together");
+  if (workspace == nullptr || ws_bytes < need)
+    return fail(TMLA_ERR_WORKSPACE_TOO_SMALL, "workspace is missing or smaller than tmla_shared_workspace_bytes()");
+  return TMLA_OK;
+}
+
 }  // namespace tmla

@@ -34,6 +34,7 @@
 
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "cdna.h"
@@ -1515,9 +1516,10 @@ constexpr int own_step_reads(int t) {
   return t < NS ? (t < 32 ? 1 : 2) : (t < NS + NV ? 2 : 0);
 }
 
-template <int DT, bool PAGED, bool PAGE_UNIFORM>
+template <int DT, bool PAGED, bool PAGE_UNIFORM, class Args = PartialArgs>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
-void mla_partial_own_kernel(PartialArgs a) {
+void mla_partial_own_kernel(Args a) {
+  constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
   constexpr int DV = 512, DQK = 576;
   constexpr int NCB = DQK / 64;   // 128-byte column blocks per row
   constexpr int NVB = DV / 64;    // ... of which hold V dims
@@ -1564,10 +1566,18 @@ void mla_partial_own_kernel(PartialArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nwg = gridDim.x;
   const int worker = worker_index(a);
-  const int head_base = blockIdx.y * 128 + wave * kHeadsPerWave;
-  const int lag_wave = __builtin_amdgcn_readfirstlane(causal_lag(a, head_base));
-  const int pre_len = __builtin_amdgcn_readfirstlane((a.fused && worker < a.batch) ? a.seqlens[worker] : 1);
-  if (a.fused && tid == 0) s_pend[0][0] = s_pend[1][0] = -1;
+  const int head_base = (SHARED ? 0 : blockIdx.y * 128) + wave * kHeadsPerWave;
+  // (SHARED: of the current item's rows, set with it)
+  int lag_wave = SHARED ? 0 : __builtin_amdgcn_readfirstlane(causal_lag(a, head_base));
+  SharedItem item{};
+  const bool fused = !SHARED && a.fused;
+  const int pre_len = __builtin_amdgcn_readfirstlane((fused && worker < a.batch) ? a.seqlens[worker] : 1);
+  if (fused && tid == 0) s_pend[0][0] = s_pend[1][0] = -1;
+  // SHARED: tokens at the end that row `local` of the item does not see
+  auto row_lag = [&](int local) __attribute__((always_inline)) {
+    const int row = item.row0 + min(local, item.rows - 1);
+    return item.causal ? causal_lag(a, row % a.num_heads) : 0;
+  };
 
   // Q rows of sequence bq for this wave's heads into V ring entry `wave` and
   // rope entry `wave`, in the KV copies' swizzled layout (heads past
@@ -1578,7 +1588,13 @@ void mla_partial_own_kernel(PartialArgs a) {
 #pragma unroll
     for (int rg = 0; rg < 4; ++rg) {
       const int hq = head_base + 8 * rg + r;
-      const char* src = a.q + ((int64_t)bq * a.q_sb + (int64_t)(hq < a.num_heads ? hq : 0) * a.q_sh) * 2 +
+      int row_b = bq, row_h = hq < a.num_heads ? hq : 0;
+      if constexpr (SHARED) {
+        const int row = item.row0 + (hq < item.rows ? hq : 0);
+        row_b = row / a.num_heads;
+        row_h = row - row_b * a.num_heads;
+      }
+      const char* src = a.q + ((int64_t)row_b * a.q_sb + (int64_t)row_h * a.q_sh) * 2 +
                         ((ln & 7) ^ piece_swizzle(r, rg)) * 16;
       static_for<NCB>([&](auto CB) __attribute__((always_inline)) {
         constexpr int cb = decltype(CB)::value;
@@ -1590,13 +1606,21 @@ void mla_partial_own_kernel(PartialArgs a) {
   };
 
   // ---- work range -------------------------------------------------------
-  WorkRange wr;
-  if (!work_range(a, worker, wr)) {
-    if (!a.fused) return;
+  WorkRange wr{};
+  int item_i = 0, sh_items = 0, sh_lo = 0, sh_hi = 0;
+  if constexpr (SHARED) {
+    const SharedHeader h = *a.header;
+    sh_items = __builtin_amdgcn_readfirstlane(h.items);
+    sh_lo = __builtin_amdgcn_readfirstlane(worker * h.chunk);
+    sh_hi = __builtin_amdgcn_readfirstlane(min(sh_lo + h.chunk, h.total));
+    if (sh_lo >= sh_hi) return;
+    item_i = __builtin_amdgcn_readfirstlane(a.worker_item[worker]);
+  } else if (!work_range(a, worker, wr)) {
+    if (!fused) return;
   }
   const int b_first = wr.b_first, tile_lo = wr.tile_lo, tile_hi = wr.tile_hi;
   const int off_first = wr.off_first, n_first = wr.n_first;
-  if (a.fused) {
+  if (fused) {
     // empty sequences worker, worker + nwg, ...: out = 0, lse = -inf
     const int lane = lane_id_fresh();
     const int hb0 = blockIdx.y * 128;
@@ -1608,7 +1632,7 @@ void mla_partial_own_kernel(PartialArgs a) {
         for (int h = hb0 + wave; h < hb0 + nh; h += 4) merge_zero(mv, bb, h, lane);
     }
   }
-  if (tile_lo >= tile_hi) return;
+  if (!SHARED && tile_lo >= tile_hi) return;
   phase_stamp(1);
 
   int b = b_first;
@@ -1616,17 +1640,42 @@ void mla_partial_own_kernel(PartialArgs a) {
   int remaining = tile_hi - tile_lo;
   int seg_global_off = off_first;
 
-  while (remaining > 0) {
-    const int n_b = b == b_first ? n_first : a.seqlens[b];
-    const int nt_b = tiles_of(n_b);
-    if (nt_b == 0) {
-      ++b;
-      continue;
+  while (SHARED ? item_i < sh_items : remaining > 0) {
+    int n_b, nt_b, t_end;
+    if constexpr (SHARED) {
+      const SharedItem* it = a.items + item_i++;
+      item.pos = __builtin_amdgcn_readfirstlane(it->pos);
+      item.tiles = __builtin_amdgcn_readfirstlane(it->tiles);
+      item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
+      item.rows = __builtin_amdgcn_readfirstlane(it->rows);
+      item.tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
+      item.causal = __builtin_amdgcn_readfirstlane(it->causal);
+      item.first_worker = __builtin_amdgcn_readfirstlane(it->first_worker);
+      item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
+      n_b = __builtin_amdgcn_readfirstlane(it->len);
+      b = __builtin_amdgcn_readfirstlane(it->seq);
+      if (item.tiles == 0) continue;
+      if (item.pos - kSegCostTiles >= sh_hi) break;
+      // tiles of the item in this range, then counted from the sequence's start
+      t_start = max(sh_lo - item.pos, 0);
+      t_end = min(item.tiles, sh_hi - item.pos);
+      if (t_start >= t_end) continue;  // only positions before its first tile
+      t_start += item.tile0;
+      t_end += item.tile0;
+      nt_b = item.tile0 + item.tiles;
+      lag_wave = __builtin_amdgcn_readfirstlane(row_lag(head_base));
+    } else {
+      n_b = b == b_first ? n_first : a.seqlens[b];
+      nt_b = tiles_of(n_b);
+      if (nt_b == 0) {
+        ++b;
+        continue;
+      }
+      t_end = min(nt_b, t_start + remaining);
     }
-    const int t_end = min(nt_b, t_start + remaining);
     const int lane = lane_id_fresh();
     const int head = head_base + (lane & 31);
-    const bool head_ok = head < a.num_heads;
+    const bool head_ok = head < (SHARED ? item.rows : a.num_heads);
     const int hi = lane >> 5;
     // S^T A operand: token lane%32, piece 2*(kc%4) + hi of column block kc/4
     int k_off_v[4];
@@ -1660,11 +1709,14 @@ void mla_partial_own_kernel(PartialArgs a) {
     seg.b = b;
     seg.t0 = t_start;
     seg.t1 = t_end;
-    {
+    if constexpr (SHARED) {
+      seg.slot = worker - item.first_worker;  // always a partial: the prefix's and the sequence's own meet in stage 2
+      seg.direct = false;
+    } else {
       const SegmentSlot ss = segment_slot(a, wr, worker, b, t_start, nt_b, seg_global_off);
       seg.slot = ss.slot;
       seg.direct = ss.direct;
-      if (a.fused && !seg.direct && wave == 0 && lane == 0) {
+      if (fused && !seg.direct && wave == 0 && lane == 0) {
         int* r = s_pend[b == b_first ? 0 : 1];
         r[0] = b;
         r[1] = ss.index;
@@ -1845,7 +1897,7 @@ void mla_partial_own_kernel(PartialArgs a) {
         if ((st + 1) * kSubTokens > n_b - lag_wave) {  // tokens past the sequence (for some head)
           const int ln = lane_id_fresh();
           const int tok0 = st * kSubTokens + 4 * (ln >> 5);
-          const int lim = n_b - causal_lag(a, head_base + (ln & 31));
+          const int lim = n_b - (SHARED ? row_lag(head_base + (ln & 31)) : causal_lag(a, head_base + (ln & 31)));
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (tok0 + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -INFINITY;
@@ -2049,7 +2101,8 @@ void mla_partial_own_kernel(PartialArgs a) {
     {
       const int ln = lane_id_fresh();
       const int hq = head_base + (ln & 31);
-      const bool hq_ok = hq < a.num_heads;
+      const int item_rows = SHARED ? item.rows : a.num_heads;
+      const bool hq_ok = hq < item_rows;
       const int h2 = ln >> 5;
       float l_a = l_run, l_b = l_run;
       swap_rows32(l_a, l_b);
@@ -2084,10 +2137,10 @@ void mla_partial_own_kernel(PartialArgs a) {
         dst = reinterpret_cast<short*>(a.out) + (int64_t)b * a.out_sb + (int64_t)head_base * a.out_sh;
         row_stride = a.out_sh;
       } else {
-        dst = a.mid_o + ((int64_t)seg.slot * a.num_heads + head_base) * DV;
+        dst = a.mid_o + ((SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + head_base) * DV;
         row_stride = DV;
       }
-      int rows = __builtin_amdgcn_readfirstlane(max(0, min(32, a.num_heads - head_base)));
+      int rows = __builtin_amdgcn_readfirstlane(max(0, min(32, item_rows - head_base)));
       // computed per segment: 32 hoisted row conditions would crowd the SGPRs
       asm volatile("" : "+s"(rows));
 #pragma unroll
@@ -2104,7 +2157,7 @@ void mla_partial_own_kernel(PartialArgs a) {
           if (a.lse) a.lse[(int64_t)b * a.num_heads + hq] = has ? lse2 * kLn2 : -INFINITY;
         }
         else
-          store_through_f32(a.mid_lse + (int64_t)seg.slot * a.num_heads + hq, lse2);
+          store_through_f32(a.mid_lse + (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + hq, lse2);
       }
       // the next segment refills the rings
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -2112,7 +2165,7 @@ void mla_partial_own_kernel(PartialArgs a) {
     }
 
     if (b == b_first) phase_stamp(4);
-    if (a.fused && !seg.direct) {
+    if (fused && !seg.direct) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       lds_barrier();
       if (wave == 0 && lane == 0) {
@@ -2122,13 +2175,14 @@ void mla_partial_own_kernel(PartialArgs a) {
       }
     }
 
+    if constexpr (SHARED) continue;
     remaining -= t_end - t_start + wr.seg_cost;  // the next sequence's start is charged here
     seg_global_off += nt_b + wr.seg_cost;
     ++b;
     t_start = 0;
   }
 
-  if (a.fused) {
+  if (fused) {
     const CoherentLoads ld{
         __builtin_amdgcn_make_buffer_rsrc(a.mid_o, 0, a.mid_o_bytes, kBufferWord3),
         __builtin_amdgcn_make_buffer_rsrc(a.mid_lse, 0, a.mid_o_bytes / 256, kBufferWord3)};
@@ -2253,6 +2307,20 @@ template <int DT, bool PAGED, bool UNI>
 hipError_t launch_partial_own_t(const PartialArgs& a, dim3 grid, hipStream_t stream) {
   hipLaunchKernelGGL((mla_partial_own_kernel<DT, PAGED, UNI>), grid, dim3(256), 0, stream, a);
   return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_partial_shared_t(const SharedArgs& a, int workers, bool uni, hipStream_t stream) {
+  if (uni)
+    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, true, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, false, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, hipStream_t stream) {
+  return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(a, workers, uni, stream)
+                            : launch_partial_shared_t<TMLA_FP16>(a, workers, uni, stream);
 }
 
 template <int DT>

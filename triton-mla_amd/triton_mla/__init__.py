@@ -7,6 +7,7 @@ from .fp8 import dequantize_kv_fp8, quantize_kv_fp8
 from .kernel import get_num_splits, mla_decode
 from .model import MLA, MLAConfig
 from .reference import mla_decode_ref, mla_decode_torch
+from .shared import mla_decode_shared
 
 __version__ = "0.1.1"
 
@@ -17,6 +18,7 @@ __all__ = [
     "get_num_splits",
     "mla_decode",
     "mla_decode_ref",
+    "mla_decode_shared",
     "mla_decode_torch",
     "quantize_kv_fp8",
 ]

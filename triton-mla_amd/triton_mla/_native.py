@@ -68,6 +68,10 @@ SIGNATURES = {
     "tmla_mla_decode_fp8_partial": (ctypes.c_int, [
         _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32,
         _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "tmla_shared_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "tmla_mla_decode_shared": (ctypes.c_int, [
+        _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32,
+        _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "tmla_mla_absorb_q": (ctypes.c_int, [
         _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp]),
     "tmla_mla_absorb_out": (ctypes.c_int, [

@@ -1,0 +1,139 @@
+"""Decode over shared prefixes: ``mla_decode_shared``.
+
+No counterpart in the reference, which reads every sequence's cache on its
+own (src/triton_mla/kernel.py:83-123). Where sequences begin with the same
+pages (samples of one prompt, a system prompt), the rows of a whole group
+attend to those pages once (csrc/mla_decode_shared.hip).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from . import kernel as _k
+
+
+def mla_decode_shared(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    block_table: torch.Tensor,
+    prefix_lens,
+    group_starts: torch.Tensor = None,
+    head_dim_v: int = 512,
+    softmax_scale: float = None,
+    return_lse: bool = False,
+    kv_scale=None,
+):
+    """``mla_decode`` of a batch whose sequences share prefixes.
+
+    The batch is cut into groups of consecutive sequences; the first tokens of
+    a group's sequences lie in the same pages, and the group attends to them
+    once. The result is ``mla_decode``'s, up to the rounding of its split
+    partials.
+
+    Args:
+        q, kv_cache, cache_seqlens, head_dim_v, softmax_scale, return_lse:
+            as ``mla_decode`` takes them (one query token a sequence, or
+            [batch, q_len, num_heads, D]), at head_dim_v 512 and rope dim 64.
+        block_table: [batch, max_blocks_per_seq] page indices (required: only
+            pages can be shared).
+        prefix_lens: tokens that the sequences of each group share: int32
+            [groups], or one int for all. The first cdiv(prefix, page_size)
+            entries of a group's rows of the block table name pages with the
+            same contents in those tokens (the same pages, normally); they are
+            read through the group's first sequence that holds a token. Less
+            than the whole may be shared: whole 64-token tiles are, and no more
+            than the shortest sequence of the group holds (sequences of length
+            0 aside), so any value is safe, up to that promise.
+        group_starts: int32 [groups + 1], ascending: group g is the sequences
+            [group_starts[g], group_starts[g + 1]); sequences outside every
+            group share nothing. None: the whole batch is one group.
+        kv_scale: not supported yet; an fp8 cache is refused.
+
+    Returns:
+        out [batch, num_heads, head_dim_v] in q.dtype (and lse [batch,
+        num_heads] float32), with the q_len dim for a 4-D q.
+    """
+    if kv_cache.dim() == 4:
+        assert kv_cache.shape[2] == 1, "MLA uses a single shared latent KV head"
+        kv_cache = kv_cache.squeeze(2)
+    multi_token = q.dim() == 4
+    q_len = 1
+    if multi_token:
+        q_len = q.shape[1]
+        assert q_len >= 1, "q must hold at least one query token"
+        if q.stride(1) != q.shape[2] * q.stride(2):
+            q = q.contiguous()
+        q = q.reshape(q.shape[0], q_len * q.shape[2], q.shape[3])
+    assert q.dim() == 3 and kv_cache.dim() == 3
+    batch, rows, d_qk = q.shape
+    num_heads = rows // q_len
+    d_rope = d_qk - head_dim_v
+    assert kv_cache.shape[-1] == d_qk
+    assert q.stride(-1) == 1 and kv_cache.stride(-1) == 1
+    if block_table is None:
+        raise ValueError("mla_decode_shared needs a paged cache (block_table): only pages can be shared")
+    if kv_cache.dtype in _k._FP8_CACHE or kv_scale is not None:
+        raise NotImplementedError("mla_decode_shared takes a bf16 or fp16 cache")
+    assert q.dtype == kv_cache.dtype
+    if q.device.type != "cuda" or kv_cache.device != q.device:
+        raise RuntimeError("triton_mla.mla_decode_shared runs on the GPU only: q and kv_cache must be "
+                           "on the same HIP device")
+    if q.dtype not in _k._DTYPES:
+        raise NotImplementedError(f"mla_decode_shared supports bf16 and fp16 inputs, got {q.dtype}")
+    if (head_dim_v, d_rope) not in _k._SUPPORTED_DIMS:
+        raise NotImplementedError(
+            f"mla_decode_shared is built for head_dim_v=512, rope_dim=64; got {head_dim_v}, {d_rope}")
+    if softmax_scale is None:
+        softmax_scale = d_qk ** -0.5
+    device = q.device
+    cache_seqlens = cache_seqlens.to(device=device, dtype=torch.int32).contiguous()
+    assert cache_seqlens.shape == (batch,), "cache_seqlens must be [batch]"
+    block_table = block_table.to(device=device, dtype=torch.int32)
+    if block_table.stride(-1) != 1:
+        block_table = block_table.contiguous()
+    assert block_table.dim() == 2 and block_table.shape[0] == batch
+    groups, starts_ptr = 1, None
+    if group_starts is not None:
+        group_starts = group_starts.to(device=device, dtype=torch.int32).contiguous()
+        assert group_starts.dim() == 1 and group_starts.shape[0] >= 2, "group_starts must be [groups + 1]"
+        groups, starts_ptr = group_starts.shape[0] - 1, group_starts.data_ptr()
+    prefix_len, prefix_ptr = 0, None
+    if torch.is_tensor(prefix_lens):
+        prefix_lens = prefix_lens.to(device=device, dtype=torch.int32).contiguous()
+        assert prefix_lens.shape == (groups,), "prefix_lens must be [groups] (or one int)"
+        prefix_ptr = prefix_lens.data_ptr()
+    else:
+        prefix_len = int(prefix_lens)
+        if not 0 <= prefix_len < 1 << 31:
+            raise ValueError("prefix_lens must be in [0, 2^31)")
+    shape = (batch, q_len, num_heads) if multi_token else (batch, num_heads)
+    out = torch.empty(*shape, head_dim_v, dtype=q.dtype, device=device)
+    lse = torch.empty(*shape, dtype=torch.float32, device=device) if return_lse else None
+    if batch:
+        if kv_cache.shape[0] == 0 or kv_cache.shape[1] == 0:
+            raise ValueError("kv_cache holds no tokens")
+        if not _k._aligned(q):
+            q = q.clone(memory_format=torch.contiguous_format)
+        if not _k._aligned(kv_cache):
+            kv_cache = kv_cache.clone(memory_format=torch.contiguous_format)
+        lib = _native.load_gil_held()  # the stream's workspace is shared by its calls
+        workers = _k._num_sms(device)
+        call = _k._CallShape()
+        call.dev_idx = device.index if device.index is not None else torch.cuda.current_device()
+        call.device = device
+        call.ws_bytes = lib.tmla_shared_workspace_bytes(batch, rows, groups, workers)
+        call.ws_alloc = max(call.ws_bytes, 16)
+        with _k._OnDevice(call.dev_idx):
+            stream = _k._raw_stream(call.dev_idx)
+            ws, ws_ptr = _k._workspace(call, stream)
+            _native.check(lib.tmla_mla_decode_shared(
+                q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1),
+                kv_cache.shape[0], kv_cache.shape[1], block_table.data_ptr(), block_table.stride(0),
+                block_table.shape[1], cache_seqlens.data_ptr(), prefix_ptr, prefix_len, starts_ptr, groups, batch,
+                q_len, num_heads, head_dim_v, d_rope, _native.DTYPE_CODE[q.dtype], float(softmax_scale), workers,
+                out.data_ptr(), out.stride(0), out.stride(-2), None if lse is None else lse.data_ptr(), ws_ptr,
+                call.ws_bytes, stream), "tmla_mla_decode_shared")
+    return (out, lse) if return_lse else out
