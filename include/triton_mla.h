@@ -536,6 +536,79 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
                            void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Page operations of a paged cache. No counterpart in the reference, which
+ * takes a block table that its caller made. Common arguments:
+ *
+ *   kv            [num_pages, page_size, row_elems] elements of elem_bytes (1, 2
+ *                 or 4), element strides (kv_stride_0, kv_stride_1, 1); rows and
+ *                 pages must not overlap. Written in place.
+ *   kv_scale      float32 scales that move with their pages: scale_cols per
+ *                 page, element strides (scale_stride_0, scale_stride_1); NULL:
+ *                 none.
+ *   table         int32 [batch, width], rows table_stride apart. An entry
+ *                 outside [0, num_pages) holds nothing. At most 2^20 rows.
+ *   refs          int32 [num_pages], how many entries hold a page; a page whose
+ *                 count is not positive is free.
+ *   new_table     [batch, width] packed; new_seqlens [batch]; new_refs
+ *                 [num_pages]: the new state (none of them an input).
+ *   workspace     tmla_pages_workspace_bytes(num_pages, batch, pairs) bytes (batch
+ *                 0 for a copy, pairs 0 for the others), 16-byte aligned, no
+ *                 initialisation.
+ *
+ * Choices go by order: the lowest free page first, rows and columns in order.
+ *
+ * tmla_pages_copy: page src[i] to page dst[i]. *refused counts the pairs left
+ * out: an id outside the pool, a destination that a later pair has too, a source
+ * that another pair writes.
+ *
+ * tmla_pages_fork: row i becomes a copy of row parents[i] (outside [0, batch):
+ * an empty row). The first copy of a row keeps all of its entries; further ones
+ * share its full pages and get a free page with a copy of a last page that is
+ * not full. Rows that no row continues release their pages, which the copies
+ * may take. *missing: the free pages lacking; if not 0, the new state equals
+ * the old and the cache is not written.
+ *
+ * tmla_pages_free: rows with ended[b] != 0 release their pages (entries -1,
+ * length 0).
+ *
+ * tmla_pages_reserve: the first cdiv(seqlens[b] + new_tokens[b], page_size)
+ * entries of row b that hold no page get one (new_tokens NULL: new_tokens_all
+ * for every row; below 0 counts as 0). *missing: the pages lacking, or columns;
+ * if not 0, the new state equals the old.
+ *
+ * tmla_pages_compact: with L pages in use (*live), those behind the first L move,
+ * in order, to the free ones among them; entries and counts follow.
+ */
+size_t tmla_pages_workspace_bytes(int64_t num_pages, int32_t batch, int32_t pairs);
+int tmla_pages_copy(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t num_pages,
+                    int32_t page_size, int32_t row_elems, int32_t elem_bytes, float* kv_scale,
+                    int64_t scale_stride_0, int64_t scale_stride_1, int32_t scale_cols,
+                    const int32_t* src, const int32_t* dst, int32_t pairs, int32_t* refused,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int tmla_pages_fork(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t num_pages,
+                    int32_t page_size, int32_t row_elems, int32_t elem_bytes, float* kv_scale,
+                    int64_t scale_stride_0, int64_t scale_stride_1, int32_t scale_cols,
+                    const int32_t* table, int64_t table_stride, int32_t batch, int32_t width,
+                    const int32_t* seqlens, const int32_t* refs, const int32_t* parents,
+                    int32_t* new_table, int32_t* new_seqlens, int32_t* new_refs, int32_t* missing,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int tmla_pages_free(const int32_t* table, int64_t table_stride, int32_t batch, int32_t width,
+                    const int32_t* seqlens, const int32_t* refs, int64_t num_pages, const uint8_t* ended,
+                    int32_t* new_table, int32_t* new_seqlens, int32_t* new_refs, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int tmla_pages_reserve(const int32_t* table, int64_t table_stride, int32_t batch, int32_t width,
+                       const int32_t* seqlens, const int32_t* refs, int64_t num_pages, int32_t page_size,
+                       const int32_t* new_tokens, int32_t new_tokens_all, int32_t* new_table,
+                       int32_t* new_refs, int32_t* missing, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int tmla_pages_compact(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t num_pages,
+                       int32_t page_size, int32_t row_elems, int32_t elem_bytes, float* kv_scale,
+                       int64_t scale_stride_0, int64_t scale_stride_1, int32_t scale_cols,
+                       const int32_t* table, int64_t table_stride, int32_t batch, int32_t width,
+                       const int32_t* refs, int32_t* new_table, int32_t* new_refs, int32_t* live,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

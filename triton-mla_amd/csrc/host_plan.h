@@ -431,4 +431,75 @@ inline int check_shared(const SharedCall& c, const void* workspace, size_t ws_by
   return TMLA_OK;
 }
 
+// ---------------------------------------------------------------------------
+// Page operations (cache_pages.hip)
+// ---------------------------------------------------------------------------
+constexpr int kPagesMaxChunks = 1024;
+constexpr int32_t kPagesMaxRows = 1 << 20;  // rows of a table
+
+// Pages per chunk of the counts: at most 1,024 chunks of at least 4,096 pages
+// (below, one chunk's pages take one workgroup less than a launch).
+inline int32_t pages_chunk(int32_t pages) {
+  const int64_t per = ((int64_t)pages + kPagesMaxChunks - 1) / kPagesMaxChunks;
+  return per < 4096 ? 4096 : (int32_t)per;
+}
+
+// Largest unit of 16, 4, 2 or 1 bytes that address, strides and row bytes allow.
+inline int32_t pages_unit(uintptr_t base, int64_t s0, int64_t s1, int64_t row_bytes) {
+  const uint64_t x = (uint64_t)base | (uint64_t)s0 | (uint64_t)s1 | (uint64_t)row_bytes;
+  return x % 16 == 0 ? 16 : x % 4 == 0 ? 4 : x % 2 == 0 ? 2 : 1;
+}
+
+inline int check_pool(int64_t pages, int32_t page_size, int32_t row_elems, int32_t elem_bytes, int64_t s0, int64_t s1) {
+  if (pages < 1 || pages > INT32_MAX - 8192) return fail(TMLA_ERR_INVALID_ARGUMENT, "num_pages must be in [1, 2^31 - 8193]");
+  if (page_size < 1 || row_elems < 1) return fail(TMLA_ERR_INVALID_ARGUMENT, "page_size and row_elems must be > 0");
+  if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)
+    return fail(TMLA_ERR_INVALID_ARGUMENT, "elem_bytes must be 1, 2 or 4");
+  const int64_t row = row_elems, page = (int64_t)page_size * row;  // elements
+  if (page * elem_bytes > INT32_MAX) return fail(TMLA_ERR_UNSUPPORTED, "a page must be smaller than 2^31 bytes");
+  // rows of a page and pages of the pool apart, or writes would meet: pages
+  // one after another, or their rows dealt out in turn
+  const int64_t r1 = page_size > 1 ? s1 : row, p0 = pages > 1 ? s0 : row;
+  if (r1 < row || p0 < row || r1 > kMaxWorkspaceBytes / page_size || p0 > kMaxWorkspaceBytes / pages ||
+      (pages > 1 && page_size > 1 && p0 < (page_size - 1) * r1 + row && r1 < (pages - 1) * p0 + row))
+    return fail(TMLA_ERR_INVALID_ARGUMENT, "pages and their rows must not overlap");
+  return TMLA_OK;
+}
+
+inline int check_tables(int32_t batch, int32_t width, int64_t pages, int32_t page_size) {
+  if (batch < 0 || width < 1) return fail(TMLA_ERR_INVALID_ARGUMENT, "batch must be >= 0 and the table's width > 0");
+  if ((int64_t)batch * width > INT32_MAX) return fail(TMLA_ERR_UNSUPPORTED, "a table must have fewer than 2^31 entries");
+  if (batch > kPagesMaxRows) return fail(TMLA_ERR_UNSUPPORTED, "batch must be at most 2^20");
+  if (pages < 1 || pages > INT32_MAX - 8192) return fail(TMLA_ERR_INVALID_ARGUMENT, "num_pages must be in [1, 2^31 - 8193]");
+  if (page_size < 1) return fail(TMLA_ERR_INVALID_ARGUMENT, "page_size must be > 0");
+  return TMLA_OK;
+}
+
+// Workspace: a flag, the chunks' counts, three values a row of the table,
+// three lists of pages and the pairs of a copy.
+struct PagesWs {
+  size_t flag, chunks, rows, ids, ids2, ids3, pairs, total;  // total 0: invalid arguments
+};
+inline PagesWs pages_ws(int64_t pages, int32_t batch, int32_t pairs) {
+  PagesWs w{0, 0, 0, 0, 0, 0, 0, 0};
+  if (pages < 1 || pages > INT32_MAX || batch < 0 || pairs < 0) return w;
+  auto al = [](int64_t x) { return (size_t)((x + 255) & ~(int64_t)255); };
+  w.chunks = 256;
+  w.rows = w.chunks + al(kPagesMaxChunks * 4);
+  w.ids = w.rows + al((int64_t)batch * 12);
+  w.ids2 = w.ids + al(pages * 4);
+  w.ids3 = w.ids2 + al(pages * 4);
+  w.pairs = w.ids3 + al(pages * 4);
+  w.total = w.pairs + al((int64_t)pairs * 8);
+  return w;
+}
+inline int check_pages_ws(int64_t pages, int32_t batch, int32_t pairs, const void* workspace, size_t bytes) {
+  const size_t need = pages_ws(pages, batch, pairs).total;
+  if (need == 0) return fail(TMLA_ERR_INVALID_ARGUMENT, "num_pages, batch and pairs must not be negative");
+  if (workspace == nullptr || bytes < need)
+    return fail(TMLA_ERR_WORKSPACE_TOO_SMALL, "workspace is missing or smaller than tmla_pages_workspace_bytes()");
+  if ((uintptr_t)workspace & 15) return fail(TMLA_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+  return TMLA_OK;
+}
+
 }  // namespace tmla

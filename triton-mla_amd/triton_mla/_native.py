@@ -72,6 +72,19 @@ SIGNATURES = {
     "tmla_mla_decode_shared": (ctypes.c_int, [
         _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32,
         _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "tmla_pages_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "tmla_pages_copy": (ctypes.c_int, [
+        _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _sz, _vp]),
+    "tmla_pages_fork": (ctypes.c_int, [
+        _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
+        _vp, _vp, _vp, _sz, _vp]),
+    "tmla_pages_free": (ctypes.c_int, [
+        _vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tmla_pages_reserve": (ctypes.c_int, [
+        _vp, _i64, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tmla_pages_compact": (ctypes.c_int, [
+        _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
+        _sz, _vp]),
     "tmla_mla_absorb_q": (ctypes.c_int, [
         _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp]),
     "tmla_mla_absorb_out": (ctypes.c_int, [
