@@ -505,6 +505,10 @@ int tmla_mla_project(const void* x, int64_t x_stride, const void* w, int64_t w_s
  *                 a sequence, query token t of row t * num_heads + h; out and
  *                 q with element strides (stride_b, stride_h, 1). lse may be
  *                 NULL.
+ *   kv_scale      NULL: kv holds elements of dtype. Otherwise it holds E4M3 codes
+ *                 (strides multiples of 16, pages of a power of two of at least
+ *                 32 tokens) and the rows of page p stand for
+ *                 e4m3(code) * kv_scale[p * scale_stride_0].
  *   prefix_lens   [num_groups] tokens that each group shares, or NULL:
  *                 prefix_len for every group. Of these, whole 64-token tiles
  *                 are shared, no more than the group's shortest sequence
@@ -528,8 +532,9 @@ int tmla_mla_project(const void* x, int64_t x_stride, const void* w, int64_t w_s
 size_t tmla_shared_workspace_bytes(int32_t batch, int32_t num_heads, int32_t num_groups, int32_t num_workers);
 int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* kv,
                            int64_t kv_stride_0, int64_t kv_stride_1, int64_t num_blocks,
-                           int32_t page_size, const int32_t* block_table, int64_t bt_stride_b,
-                           int32_t bt_cols, const int32_t* cache_seqlens, const int32_t* prefix_lens,
+                           int32_t page_size, const float* kv_scale, int64_t scale_stride_0,
+                           const int32_t* block_table, int64_t bt_stride_b, int32_t bt_cols,
+                           const int32_t* cache_seqlens, const int32_t* prefix_lens,
                            int32_t prefix_len, const int32_t* group_starts, int32_t num_groups,
                            int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim_v,
                            int32_t rope_dim, int32_t dtype, float softmax_scale, int32_t num_workers,

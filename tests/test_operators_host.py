@@ -59,7 +59,7 @@ FAKE = 1 << 20  # a non-null, aligned address that no refused call reads
 
 
 def _shared(lib, **kw):
-    a = dict(q=FAKE, q_sb=16 * 576, q_sh=576, kv=FAKE, s0=64 * 576, s1=576, blocks=4, page=64, bt=FAKE, bt_s=2,
+    a = dict(q=FAKE, q_sb=16 * 576, q_sh=576, kv=FAKE, s0=64 * 576, s1=576, blocks=4, page=64, kv_scale=None, sc_s0=0, bt=FAKE, bt_s=2,
              bt_cols=2, lens=FAKE, prefix=None, prefix_len=64, starts=None, groups=1, batch=2, q_len=1, heads=16,
              dv=512, dr=64, dtype=0, scale=0.1, workers=256, out=FAKE, out_sb=16 * 512, out_sh=512, lse=None, ws=FAKE,
              ws_bytes=1 << 40, stream=None)
@@ -77,6 +77,8 @@ def _shared(lib, **kw):
     ({"q": None}, 1, b"null"), ({"bt": None}, 1, b"null"), ({"lens": None}, 1, b"null"), ({"out": None}, 1, b"null"),
     ({"q": FAKE + 2}, 1, b"aligned"), ({"ws": FAKE + 4}, 1, b"aligned"), ({"out_sh": 513}, 1, b"multiples of 8"),
     ({"ws": None}, 3, b"workspace"), ({"ws_bytes": 1000}, 3, b"workspace"),
+    ({"kv_scale": FAKE, "s1": 584}, 1, b"multiples of 16"), ({"kv_scale": FAKE + 2}, 1, b"aligned"),
+    ({"kv_scale": FAKE, "page": 16}, 2, b"32 tokens"), ({"kv_scale": FAKE, "page": 96}, 2, b"32 tokens"),
     ({"heads": 262141}, 2, b"262140"), ({"batch": 1 << 28}, 2, b"too large"),
     ({"bt_cols": 1 << 30, "batch": 4096}, 2, b"too large"),
 ])

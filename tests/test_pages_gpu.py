@@ -477,12 +477,14 @@ def test_serving_run(gpu, fp8):
     keeps each sequence's rows on its own."""
     import triton_mla
 
-    if fp8:
-        pytest.skip("mla_decode_shared takes a 16-bit cache")
     rng = random.Random(11)
     batch, heads, page, pages, width = 6, 16, 64, 64, 16
     g = torch.Generator(device="cuda").manual_seed(3)
     kv = torch.zeros(pages, page, 576, dtype=torch.bfloat16, device="cuda")
+    scale = None
+    if fp8:  # codes of 1/8, and one scale a page that moves with it
+        kv = torch.zeros(pages, page, 576, dtype=torch.uint8, device="cuda")
+        scale = torch.full((pages,), 0.125, device="cuda")
     table = torch.full((batch, width), -1, dtype=I32, device="cuda")
     lens = torch.zeros(batch, dtype=I32, device="cuda")
     refs = torch.zeros(pages, dtype=I32, device="cuda")
@@ -494,16 +496,19 @@ def test_serving_run(gpu, fp8):
         assert missing.item() == 0
         for b, n in enumerate(counts):
             rows = torch.randn(n, 576, generator=g, device="cuda", dtype=torch.bfloat16)
+            codes = (rows.float() * 8).to(torch.float8_e4m3fn)
             for j in range(n):
                 t = kept[b].shape[0] + j
-                kv[table[b, t // page].long(), t % page] = rows[j]
+                kv[table[b, t // page].long(), t % page] = codes[j].view(torch.uint8) if fp8 else rows[j]
+            if fp8:  # (three bits and a power of two: exact in bf16)
+                rows = (codes.float() / 8).to(torch.bfloat16)
             kept[b] = torch.cat([kept[b], rows])
         lens = lens + cuda(counts)
 
     def decode(prefix):
         q = torch.randn(batch, heads, 576, generator=g, device="cuda", dtype=torch.bfloat16)
         shared, lse = triton_mla.mla_decode_shared(q, kv, lens, table, prefix, softmax_scale=192 ** -0.5,
-                                                   return_lse=True)
+                                                   return_lse=True, kv_scale=scale)
         dense = torch.zeros(batch, max(k.shape[0] for k in kept), 576, dtype=torch.bfloat16, device="cuda")
         for b, k in enumerate(kept):
             dense[b, :k.shape[0]] = k
@@ -516,7 +521,7 @@ def test_serving_run(gpu, fp8):
 
     append([331] + [0] * (batch - 1))
     parents = [0] * batch
-    table, lens, refs, missing = triton_mla.fork_sequences(kv, table, lens, refs, cuda(parents))
+    table, lens, refs, missing = triton_mla.fork_sequences(kv, table, lens, refs, cuda(parents), scale)
     assert missing.item() == 0
     kept = [kept[0].clone() for _ in range(batch)]
     assert refs.max().item() == batch
@@ -524,15 +529,16 @@ def test_serving_run(gpu, fp8):
         append([rng.choice([1, 1, 40]) for _ in range(batch)])
         decode(320)
         parents = [rng.randrange(batch) for _ in range(batch)]
-        table, lens, refs, missing = triton_mla.fork_sequences(kv, table, lens, refs, cuda(parents))
+        table, lens, refs, missing = triton_mla.fork_sequences(kv, table, lens, refs, cuda(parents), scale)
         assert missing.item() == 0
         kept = [kept[p].clone() for p in parents]
     ended = torch.tensor([True, False] * 3, device="cuda")
     table, lens, refs = triton_mla.free_sequences(table, lens, refs, ended)
     kept = [k[:0] if e else k for k, e in zip(kept, ended.tolist())]
     q, out, lse = decode(320)
-    table, refs, live = triton_mla.compact_pages(kv, table, refs)
+    table, refs, live = triton_mla.compact_pages(kv, table, refs, scale)
     assert (refs[live.item():] == 0).all() and (refs[:live.item()] > 0).all()
     kv = kv[:live.item()].clone()  # the rest of the pool can go
-    again = triton_mla.mla_decode_shared(q, kv, lens, table, 320, softmax_scale=192 ** -0.5, return_lse=True)
+    again = triton_mla.mla_decode_shared(q, kv, lens, table, 320, softmax_scale=192 ** -0.5, return_lse=True,
+                                         kv_scale=scale[:live.item()] if fp8 else None)
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)

@@ -136,6 +136,55 @@ def test_against_float64(gpu, name):
     check(args, *run(args))
 
 
+@pytest.mark.parametrize("granularity", ["page", "tensor", "number"])
+@pytest.mark.parametrize("name", ["one_group", "rows_past_a_block", "all_heads", "more_heads_than_a_block",
+                                  "large_pages", "padded_rows", "two_tokens", "long", "nothing_of_its_own"])
+def test_fp8_against_float64(gpu, name, granularity):
+    """The codes stand for e4m3 * scale exactly, so the 16-bit bounds hold with
+    one rounding more: the probabilities take the page's scale (float32, then
+    the same rounding), the partials and the result theirs."""
+    import triton_mla
+
+    sizes, prefixes, own, heads, page, dtype, q_len, empty = CASES[name]
+    args = build(sizes, prefixes, own, heads, page, dtype, q_len, empty=empty)
+    # pages of different magnitudes
+    kv = args["kv_cache"].float() * torch.rand(args["kv_cache"].shape[0], 1, 1, device="cuda") + 0.01
+    codes, scale = triton_mla.quantize_kv_fp8(kv, "page" if granularity == "page" else "tensor")
+    values = triton_mla.dequantize_kv_fp8(codes, scale).double()
+    out, lse = run({**args, "kv_cache": codes.view(torch.uint8) if granularity == "tensor" else codes},
+                   kv_scale=float(scale) if granularity == "number" else scale)
+    check({**args, "kv_cache": codes}, out, lse, kv=values)
+
+
+def test_fp8_strides_and_zero_scales(gpu):
+    import triton_mla
+
+    args = build([3], [320], [1, 64, 100], 16)
+    codes, scale = triton_mla.quantize_kv_fp8(args["kv_cache"], "page")
+    scale[args["block_table"][0, 1].long()] = 0.0  # a page of zeros, for all of the group
+    want = run({**args, "kv_cache": codes}, kv_scale=scale)
+    check(args, *want, kv=triton_mla.dequantize_kv_fp8(codes, scale).double())
+    wide = torch.zeros(codes.shape[0], 70, 592, dtype=torch.uint8, device="cuda")
+    wide[:, :64, :576] = codes.view(torch.uint8)
+    scales = torch.zeros(codes.shape[0], 3, device="cuda")
+    scales[:, 1] = scale
+    got = run({**args, "kv_cache": wide[:, :64, :576]}, kv_scale=scales[:, 1])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_fp8_refusals(gpu):
+    args = build([3], [320], [1, 64, 100], 16)
+    codes = args["kv_cache"].to(torch.float8_e4m3fn)
+    with pytest.raises(ValueError):
+        run({**args, "kv_cache": codes})
+    with pytest.raises(NotImplementedError):  # per token
+        run({**args, "kv_cache": codes}, kv_scale=torch.ones(codes.shape[:2], device="cuda"))
+    with pytest.raises(NotImplementedError):  # small pages
+        run({**args, "kv_cache": codes.view(-1, 16, 576)}, kv_scale=1.0)
+    with pytest.raises(AssertionError):
+        run(args, kv_scale=1.0)
+
+
 def test_prefix_as_one_number_and_one_group(gpu):
     args = build([4], [320], [1, 64, 65, 130], 16)
     want = run(args)

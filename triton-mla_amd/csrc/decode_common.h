@@ -459,6 +459,59 @@ __device__ __forceinline__ void sequence_slots(const Lens& len_of, int batch, in
   }
 }
 
+// A worker's way along the items of a SharedArgs call.
+struct SharedWalk {
+  int next, items;  // next item, and their number
+  int lo, hi;       // the worker's positions
+};
+__device__ __forceinline__ bool shared_begin(const SharedArgs& a, int worker, SharedWalk& w) {
+  const SharedHeader h = *a.header;
+  w.items = __builtin_amdgcn_readfirstlane(h.items);
+  w.lo = __builtin_amdgcn_readfirstlane(worker * h.chunk);
+  w.hi = __builtin_amdgcn_readfirstlane(min(w.lo + h.chunk, h.total));
+  if (w.lo >= w.hi) return false;
+  w.next = __builtin_amdgcn_readfirstlane(a.worker_item[worker]);
+  return true;
+}
+// The next item that has tiles in the worker's range: those tiles, counted
+// from the start of its sequence, the sequence and its tokens. False at the
+// range's end.
+__device__ __forceinline__ bool shared_next(const SharedArgs& a, SharedWalk& w, SharedItem& item, int& b, int& n_b,
+                                            int& t_start, int& t_end) {
+  while (w.next < w.items) {
+    const SharedItem* it = a.items + w.next++;
+    const int pos = __builtin_amdgcn_readfirstlane(it->pos);
+    const int tiles = __builtin_amdgcn_readfirstlane(it->tiles);
+    const int tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
+    item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
+    item.rows = __builtin_amdgcn_readfirstlane(it->rows);
+    item.causal = __builtin_amdgcn_readfirstlane(it->causal);
+    item.first_worker = __builtin_amdgcn_readfirstlane(it->first_worker);
+    item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
+    n_b = __builtin_amdgcn_readfirstlane(it->len);
+    b = __builtin_amdgcn_readfirstlane(it->seq);
+    if (tiles == 0) continue;
+    if (pos - kSegCostTiles >= w.hi) return false;
+    t_start = max(w.lo - pos, 0);
+    t_end = min(tiles, w.hi - pos);
+    if (t_start >= t_end) continue;  // only positions before its first tile
+    t_start += tile0;
+    t_end += tile0;
+    return true;
+  }
+  return false;
+}
+// Query row `local` of the item (past its rows: the last one): its sequence
+// and its place there, and the tokens at the end that it does not see.
+__device__ __forceinline__ int2 shared_row(const SharedArgs& a, const SharedItem& item, int local) {
+  const int row = item.row0 + min(local, item.rows - 1);
+  const int b = row / a.num_heads;
+  return make_int2(b, row - b * a.num_heads);
+}
+__device__ __forceinline__ int shared_lag(const SharedArgs& a, const SharedItem& item, int local) {
+  return item.causal ? causal_lag(a, shared_row(a, item, local).y) : 0;
+}
+
 // Stage 1 over an fp8 cache (mla_decode_fp8.hip): grid = (workers, head
 // groups of 16); dtype is the element type of q and out.
 hipError_t launch_partial_fp8(const PartialArgs& a, dim3 grid, int dtype, bool paged, hipStream_t stream);
@@ -468,7 +521,7 @@ hipError_t launch_partial_fp8(const PartialArgs& a, dim3 grid, int dtype, bool p
 hipError_t launch_partial_g16(const PartialArgs& a, dim3 grid, int dtype, bool paged, hipStream_t stream);
 
 // Stage 1 over shared prefixes (mla_decode.hip): grid = workers; uni: pages
-// of a power of two of whole 32-token sub-tiles.
-hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, hipStream_t stream);
+// of a power of two of whole 32-token sub-tiles (an fp8 cache needs them).
+hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, bool fp8, hipStream_t stream);
 
 }  // namespace tmla

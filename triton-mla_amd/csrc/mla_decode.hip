@@ -427,9 +427,11 @@ struct Segment {
 // workgroup; the page's scale multiplies the scores (folded into the softmax
 // scale) and the probabilities before their rounding. The V ring has three
 // entries and the rope ring two, which makes room for two staging entries.
-template <int DT, int DV, int DR, int NHB, bool PAGED, bool PAGE_UNIFORM, bool F8 = false>
+template <int DT, int DV, int DR, int NHB, bool PAGED, bool PAGE_UNIFORM, bool F8 = false, class Args = PartialArgs>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
-void mla_partial_kernel(PartialArgs a) {
+void mla_partial_kernel(Args a) {
+  constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
+  static_assert(!SHARED || (F8 && NHB == 4), "shared prefixes: 128 rows a workgroup (16-bit caches: mla_partial_own_kernel)");
   constexpr int DQK = DV + DR;
   static_assert(DQK % 64 == 0 && DV % 64 == 0, "row must be whole 128-byte blocks");
   constexpr int NCB = DQK / 64;           // 128-byte column blocks per row
@@ -487,15 +489,18 @@ void mla_partial_kernel(PartialArgs a) {
   const int nwg = gridDim.x;
   const int worker = worker_index(a);
   const bool s_owner = NHB == 4 || wave < NHB;  // runs S and the softmax of head block `wave`
-  const int head_base = blockIdx.y * (kHeadsPerWave * NHB) + wave * kHeadsPerWave;
+  const int head_base = (SHARED ? 0 : blockIdx.y * (kHeadsPerWave * NHB)) + wave * kHeadsPerWave;
   // the wave's first head has its earliest query token: the most tokens unseen
-  const int lag_wave = __builtin_amdgcn_readfirstlane(causal_lag(a, head_base));
+  // (SHARED: of the current item's rows, set with it)
+  int lag_wave = SHARED ? 0 : __builtin_amdgcn_readfirstlane(causal_lag(a, head_base));
+  SharedItem item{};
+  const bool fused = !SHARED && a.fused;
   // fused merge: this worker clears sequences worker, worker + nwg, ... when
   // they are empty; the first length is requested now, used at the end
-  const int pre_len = __builtin_amdgcn_readfirstlane((a.fused && worker < a.batch) ? a.seqlens[worker] : 1);
+  const int pre_len = __builtin_amdgcn_readfirstlane((fused && worker < a.batch) ? a.seqlens[worker] : 1);
   // split segments awaiting their merge: at most the first (record 0) and
   // the last (record 1) segment of the worker's range; b < 0 = none
-  if (a.fused && tid == 0) s_pend[0][0] = s_pend[1][0] = -1;
+  if (fused && tid == 0) s_pend[0][0] = s_pend[1][0] = -1;
 
   // Q rows of sequence bq for this wave's heads into LDS (the KV copies'
   // swizzled layout; heads past num_heads copy head 0's row): V part at qv,
@@ -515,7 +520,13 @@ void mla_partial_kernel(PartialArgs a) {
 #pragma unroll
     for (int rg = 0; rg < 4; ++rg) {
       const int hq = head_base + 8 * rg + r;
-      const char* src = a.q + ((int64_t)bq * a.q_sb + (int64_t)(hq < a.num_heads ? hq : 0) * a.q_sh) * 2 +
+      int row_b = bq, row_h = hq < a.num_heads ? hq : 0;
+      if constexpr (SHARED) {
+        const int2 row = shared_row(a, item, hq);
+        row_b = row.x;
+        row_h = row.y;
+      }
+      const char* src = a.q + ((int64_t)row_b * a.q_sb + (int64_t)row_h * a.q_sh) * 2 +
                         ((ln & 7) ^ piece_swizzle(r, rg)) * 16;
       static_for<NCB>([&](auto CB) __attribute__((always_inline)) {
         constexpr int cb = decltype(CB)::value;
@@ -527,13 +538,16 @@ void mla_partial_kernel(PartialArgs a) {
   };
 
   // ---- work range -------------------------------------------------------
-  WorkRange wr;
-  if (!work_range(a, worker, wr)) {
-    if (!a.fused) return;  // (the fused tail still clears empty sequences)
+  WorkRange wr{};
+  SharedWalk walk{};
+  if constexpr (SHARED) {
+    if (!shared_begin(a, worker, walk)) return;
+  } else if (!work_range(a, worker, wr)) {
+    if (!fused) return;  // (the fused tail still clears empty sequences)
   }
   const int b_first = wr.b_first, tile_lo = wr.tile_lo, tile_hi = wr.tile_hi;
   const int off_first = wr.off_first, n_first = wr.n_first;
-  if (a.fused) {
+  if (fused) {
     // empty sequences worker, worker + nwg, ...: out = 0, lse = -inf
     // (kernel.py:126-128, 178-181); the first length was requested at entry
     const int lane = lane_id_fresh();
@@ -546,7 +560,7 @@ void mla_partial_kernel(PartialArgs a) {
         for (int h = hb0 + wave; h < hb0 + nh; h += 4) merge_zero(mv, bb, h, lane);
     }
   }
-  if (tile_lo >= tile_hi) return;
+  if (!SHARED && tile_lo >= tile_hi) return;
   phase_stamp(1);
 
   // ---- segments -----------------------------------------------------------
@@ -555,14 +569,20 @@ void mla_partial_kernel(PartialArgs a) {
   int remaining = tile_hi - tile_lo;  // tiles left in this worker's range
   int seg_global_off = off_first;     // balanced mode: tile offset of b
 
-  while (remaining > 0) {
-    const int n_b = b == b_first ? n_first : a.seqlens[b];
-    const int nt_b = tiles_of(n_b);
-    if (nt_b == 0) {  // only possible in balanced mode between sequences
-      ++b;
-      continue;
+  while (SHARED || remaining > 0) {
+    int n_b, nt_b = 0, t_end;
+    if constexpr (SHARED) {
+      if (!shared_next(a, walk, item, b, n_b, t_start, t_end)) break;
+      lag_wave = __builtin_amdgcn_readfirstlane(shared_lag(a, item, head_base));
+    } else {
+      n_b = b == b_first ? n_first : a.seqlens[b];
+      nt_b = tiles_of(n_b);
+      if (nt_b == 0) {  // only possible in balanced mode between sequences
+        ++b;
+        continue;
+      }
+      t_end = min(nt_b, t_start + remaining);
     }
-    const int t_end = min(nt_b, t_start + remaining);
     // this segment's lane-derived values (recomputed per segment, see
     // lane_id_fresh)
     const int lane = lane_id_fresh();
@@ -611,13 +631,16 @@ void mla_partial_kernel(PartialArgs a) {
     seg.b = b;
     seg.t0 = t_start;
     seg.t1 = t_end;
-    {
+    if constexpr (SHARED) {
+      seg.slot = worker - item.first_worker;  // always a partial
+      seg.direct = false;
+    } else {
       const SegmentSlot ss = segment_slot(a, wr, worker, b, t_start, nt_b, seg_global_off);
       seg.slot = ss.slot;
       seg.direct = ss.direct;
       // fused merge record: b, this worker's index among b's workers, their
       // count, b's first slot
-      if (a.fused && !seg.direct && wave == 0 && lane == 0) {
+      if (fused && !seg.direct && wave == 0 && lane == 0) {
         int* r = s_pend[b == b_first ? 0 : 1];
         r[0] = b;
         r[1] = ss.index;
@@ -1196,9 +1219,13 @@ void mla_partial_kernel(PartialArgs a) {
             if (!full) {
               const int tok0 = st_s * kSubTokens + 4 * hi;
               const float off = c >= 0.0f ? -INFINITY : INFINITY;
+              auto lag = [&]() __attribute__((always_inline)) {
+                if constexpr (SHARED) return shared_lag(a, item, head_base + (lane_id_fresh() & 31));
+                else return causal_lag(a, head_base + (lane_id_fresh() & 31));
+              };
 #pragma unroll
               for (int r = 0; r < 16; ++r)
-                if (tok0 + 8 * (r >> 2) + (r & 3) >= n_b - causal_lag(a, head_base + (lane_id_fresh() & 31))) s[r] = off;
+                if (tok0 + 8 * (r >> 2) + (r & 3) >= n_b - lag()) s[r] = off;
             }
             pin_f16(s);
           } else if constexpr (j == 1) {  // reference max
@@ -1312,7 +1339,8 @@ void mla_partial_kernel(PartialArgs a) {
     {
       const int lane = lane_id_fresh();  // (see lane_id_fresh)
       const int head = head_base + (lane & 31);
-      const bool head_ok = s_owner && head < a.num_heads;
+      const int item_rows = SHARED ? item.rows : a.num_heads;
+      const bool head_ok = s_owner && head < item_rows;
       const int hi = lane >> 5;
       const float l_tot = l_run + __shfl_xor(l_run, 32);
       const bool has = l_tot > 0.0f;
@@ -1350,11 +1378,11 @@ void mla_partial_kernel(PartialArgs a) {
         } else {
           // the partial is a convex combination of cache rows, so it fits the
           // input dtype; it is stored there (half the bytes of float32)
-          dst = a.mid_o + ((int64_t)seg.slot * a.num_heads + head_base) * DV;
+          dst = a.mid_o + ((SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + head_base) * DV;
           row_stride = DV;
         }
         // wave-uniform; only the waves that own a head block hold staged rows
-        int rows = __builtin_amdgcn_readfirstlane(wave < NHB ? min(32, a.num_heads - head_base) : 0);
+        int rows = __builtin_amdgcn_readfirstlane(wave < NHB ? min(32, item_rows - head_base) : 0);
         // computed per segment: 32 hoisted row conditions would crowd the SGPRs
         asm volatile("" : "+s"(rows));
         const char LDS_AS* obuf = lds + wave * 32 * OPITCH;
@@ -1374,7 +1402,7 @@ void mla_partial_kernel(PartialArgs a) {
             if (a.lse) a.lse[(int64_t)b * a.num_heads + head] = has ? lse2 * kLn2 : -INFINITY;
           }
           else
-            store_through_f32(a.mid_lse + (int64_t)seg.slot * a.num_heads + head, lse2);
+            store_through_f32(a.mid_lse + (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + head, lse2);
         }
         // the next segment refills the rings
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1383,7 +1411,7 @@ void mla_partial_kernel(PartialArgs a) {
     }
 
     if (b == b_first) phase_stamp(4);
-    if (a.fused && !seg.direct) {
+    if (fused && !seg.direct) {
       // every wave's write-through partial row and lse stores have
       // completed before the arrival
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1395,13 +1423,14 @@ void mla_partial_kernel(PartialArgs a) {
       }
     }
 
+    if constexpr (SHARED) continue;
     remaining -= t_end - t_start + wr.seg_cost;  // the next sequence's start is charged here
     seg_global_off += nt_b + wr.seg_cost;
     ++b;
     t_start = 0;
   }
 
-  if (a.fused) {
+  if (fused) {
     const CoherentLoads ld{
         __builtin_amdgcn_make_buffer_rsrc(a.mid_o, 0, a.mid_o_bytes, kBufferWord3),
         __builtin_amdgcn_make_buffer_rsrc(a.mid_lse, 0, a.mid_o_bytes / 256, kBufferWord3)};
@@ -1573,11 +1602,6 @@ void mla_partial_own_kernel(Args a) {
   const bool fused = !SHARED && a.fused;
   const int pre_len = __builtin_amdgcn_readfirstlane((fused && worker < a.batch) ? a.seqlens[worker] : 1);
   if (fused && tid == 0) s_pend[0][0] = s_pend[1][0] = -1;
-  // SHARED: tokens at the end that row `local` of the item does not see
-  auto row_lag = [&](int local) __attribute__((always_inline)) {
-    const int row = item.row0 + min(local, item.rows - 1);
-    return item.causal ? causal_lag(a, row % a.num_heads) : 0;
-  };
 
   // Q rows of sequence bq for this wave's heads into V ring entry `wave` and
   // rope entry `wave`, in the KV copies' swizzled layout (heads past
@@ -1590,9 +1614,9 @@ void mla_partial_own_kernel(Args a) {
       const int hq = head_base + 8 * rg + r;
       int row_b = bq, row_h = hq < a.num_heads ? hq : 0;
       if constexpr (SHARED) {
-        const int row = item.row0 + (hq < item.rows ? hq : 0);
-        row_b = row / a.num_heads;
-        row_h = row - row_b * a.num_heads;
+        const int2 row = shared_row(a, item, hq);
+        row_b = row.x;
+        row_h = row.y;
       }
       const char* src = a.q + ((int64_t)row_b * a.q_sb + (int64_t)row_h * a.q_sh) * 2 +
                         ((ln & 7) ^ piece_swizzle(r, rg)) * 16;
@@ -1607,14 +1631,9 @@ void mla_partial_own_kernel(Args a) {
 
   // ---- work range -------------------------------------------------------
   WorkRange wr{};
-  int item_i = 0, sh_items = 0, sh_lo = 0, sh_hi = 0;
+  SharedWalk walk{};
   if constexpr (SHARED) {
-    const SharedHeader h = *a.header;
-    sh_items = __builtin_amdgcn_readfirstlane(h.items);
-    sh_lo = __builtin_amdgcn_readfirstlane(worker * h.chunk);
-    sh_hi = __builtin_amdgcn_readfirstlane(min(sh_lo + h.chunk, h.total));
-    if (sh_lo >= sh_hi) return;
-    item_i = __builtin_amdgcn_readfirstlane(a.worker_item[worker]);
+    if (!shared_begin(a, worker, walk)) return;
   } else if (!work_range(a, worker, wr)) {
     if (!fused) return;
   }
@@ -1640,30 +1659,11 @@ void mla_partial_own_kernel(Args a) {
   int remaining = tile_hi - tile_lo;
   int seg_global_off = off_first;
 
-  while (SHARED ? item_i < sh_items : remaining > 0) {
-    int n_b, nt_b, t_end;
+  while (SHARED || remaining > 0) {
+    int n_b, nt_b = 0, t_end;
     if constexpr (SHARED) {
-      const SharedItem* it = a.items + item_i++;
-      item.pos = __builtin_amdgcn_readfirstlane(it->pos);
-      item.tiles = __builtin_amdgcn_readfirstlane(it->tiles);
-      item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
-      item.rows = __builtin_amdgcn_readfirstlane(it->rows);
-      item.tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
-      item.causal = __builtin_amdgcn_readfirstlane(it->causal);
-      item.first_worker = __builtin_amdgcn_readfirstlane(it->first_worker);
-      item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
-      n_b = __builtin_amdgcn_readfirstlane(it->len);
-      b = __builtin_amdgcn_readfirstlane(it->seq);
-      if (item.tiles == 0) continue;
-      if (item.pos - kSegCostTiles >= sh_hi) break;
-      // tiles of the item in this range, then counted from the sequence's start
-      t_start = max(sh_lo - item.pos, 0);
-      t_end = min(item.tiles, sh_hi - item.pos);
-      if (t_start >= t_end) continue;  // only positions before its first tile
-      t_start += item.tile0;
-      t_end += item.tile0;
-      nt_b = item.tile0 + item.tiles;
-      lag_wave = __builtin_amdgcn_readfirstlane(row_lag(head_base));
+      if (!shared_next(a, walk, item, b, n_b, t_start, t_end)) break;
+      lag_wave = __builtin_amdgcn_readfirstlane(shared_lag(a, item, head_base));
     } else {
       n_b = b == b_first ? n_first : a.seqlens[b];
       nt_b = tiles_of(n_b);
@@ -1897,7 +1897,10 @@ void mla_partial_own_kernel(Args a) {
         if ((st + 1) * kSubTokens > n_b - lag_wave) {  // tokens past the sequence (for some head)
           const int ln = lane_id_fresh();
           const int tok0 = st * kSubTokens + 4 * (ln >> 5);
-          const int lim = n_b - (SHARED ? row_lag(head_base + (ln & 31)) : causal_lag(a, head_base + (ln & 31)));
+          int lag;
+          if constexpr (SHARED) lag = shared_lag(a, item, head_base + (ln & 31));
+          else lag = causal_lag(a, head_base + (ln & 31));
+          const int lim = n_b - lag;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (tok0 + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -INFINITY;
@@ -2310,17 +2313,20 @@ hipError_t launch_partial_own_t(const PartialArgs& a, dim3 grid, hipStream_t str
 }
 
 template <int DT>
-hipError_t launch_partial_shared_t(const SharedArgs& a, int workers, bool uni, hipStream_t stream) {
-  if (uni)
+hipError_t launch_partial_shared_t(const SharedArgs& a, int workers, bool uni, bool fp8, hipStream_t stream) {
+  if (fp8)
+    hipLaunchKernelGGL((mla_partial_kernel<DT, 512, 64, 4, true, true, true, SharedArgs>), dim3(workers), dim3(256), 0,
+                       stream, a);
+  else if (uni)
     hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, true, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, false, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
-hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, hipStream_t stream) {
-  return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(a, workers, uni, stream)
-                            : launch_partial_shared_t<TMLA_FP16>(a, workers, uni, stream);
+hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, bool fp8, hipStream_t stream) {
+  return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(a, workers, uni, fp8, stream)
+                            : launch_partial_shared_t<TMLA_FP16>(a, workers, uni, fp8, stream);
 }
 
 template <int DT>

@@ -303,7 +303,8 @@ size_t tmla_shared_workspace_bytes(int32_t batch, int32_t num_heads, int32_t num
 }
 
 int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* kv, int64_t kv_stride_0,
-                           int64_t kv_stride_1, int64_t num_blocks, int32_t page_size, const int32_t* block_table,
+                           int64_t kv_stride_1, int64_t num_blocks, int32_t page_size, const float* kv_scale,
+                           int64_t scale_stride_0, const int32_t* block_table,
                            int64_t bt_stride_b, int32_t bt_cols, const int32_t* cache_seqlens,
                            const int32_t* prefix_lens, int32_t prefix_len, const int32_t* group_starts,
                            int32_t num_groups, int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim_v,
@@ -323,6 +324,13 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
   if ((q_stride_b | q_stride_h | kv_stride_0 | kv_stride_1 | out_stride_b | out_stride_h) & 7)
     return fail(TMLA_ERR_INVALID_ARGUMENT, "strides must be multiples of 8 elements");
 
+  const bool fp8 = kv_scale != nullptr;
+  if (fp8) {
+    if (((uintptr_t)kv_scale & 3) || ((kv_stride_0 | kv_stride_1) & 15))
+      return fail(TMLA_ERR_INVALID_ARGUMENT, "kv_scale must be 4-byte aligned, fp8 cache strides multiples of 16");
+    if (page_size % 32 || (page_size & (page_size - 1)))
+      return fail(TMLA_ERR_UNSUPPORTED, "an fp8 cache needs pages of a power of two of at least 32 tokens");
+  }
   const int32_t rows = q_len * num_heads;
   const SharedWs w = shared_ws(batch, rows, num_groups, num_workers);
   char* ws = static_cast<char*>(workspace);
@@ -351,8 +359,8 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
   a.q_sb = q_stride_b;
   a.q_sh = q_stride_h;
   a.kv = static_cast<const char*>(kv);
-  a.kv_s0 = kv_stride_0 * 2;
-  a.kv_s1 = kv_stride_1 * 2;
+  a.kv_s0 = kv_stride_0 * (fp8 ? 1 : 2);
+  a.kv_s1 = kv_stride_1 * (fp8 ? 1 : 2);
   a.num_blocks = num_blocks;
   a.max_page = (int32_t)(num_blocks - 1 < INT32_MAX ? num_blocks - 1 : INT32_MAX);
   a.page_size = page_size;
@@ -375,8 +383,12 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
   a.items = p.items;
   a.worker_item = p.worker_item;
   const bool uni = page_size % 32 == 0 && a.page_shift >= 0;
-  e = launch_partial_shared(a, num_workers, dtype, uni, s);
-  if (e != hipSuccess) return hip_fail(e, "mla_partial_own_kernel launch");
+  if (fp8) {
+    a.kv_scale = kv_scale;
+    a.sc_s0 = scale_stride_0;
+  }
+  e = launch_partial_shared(a, num_workers, dtype, uni, fp8, s);
+  if (e != hipSuccess) return hip_fail(e, "stage 1 launch");
 
   const SharedCombineArgs ca{p.header, p.items, p.seq_info, a.mid_o, a.mid_lse, batch, rows,
                              static_cast<char*>(out), out_stride_b, out_stride_h, lse};

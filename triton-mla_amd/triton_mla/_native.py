@@ -70,8 +70,8 @@ SIGNATURES = {
         _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "tmla_shared_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "tmla_mla_decode_shared": (ctypes.c_int, [
-        _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32,
-        _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+        _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32,
+        _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "tmla_pages_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "tmla_pages_copy": (ctypes.c_int, [
         _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _sz, _vp]),

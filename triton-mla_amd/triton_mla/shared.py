@@ -50,7 +50,9 @@ def mla_decode_shared(
         group_starts: int32 [groups + 1], ascending: group g is the sequences
             [group_starts[g], group_starts[g + 1]); sequences outside every
             group share nothing. None: the whole batch is one group.
-        kv_scale: not supported yet; an fp8 cache is refused.
+        kv_scale: scales of an fp8 cache, as ``mla_decode`` takes them, one per
+            page or one for the whole cache (scales per token are refused), on
+            pages of a power of two of at least 32 tokens.
 
     Returns:
         out [batch, num_heads, head_dim_v] in q.dtype (and lse [batch,
@@ -75,9 +77,20 @@ def mla_decode_shared(
     assert q.stride(-1) == 1 and kv_cache.stride(-1) == 1
     if block_table is None:
         raise ValueError("mla_decode_shared needs a paged cache (block_table): only pages can be shared")
-    if kv_cache.dtype in _k._FP8_CACHE or kv_scale is not None:
-        raise NotImplementedError("mla_decode_shared takes a bf16 or fp16 cache")
-    assert q.dtype == kv_cache.dtype
+    fp8 = kv_cache.dtype in _k._FP8_CACHE
+    if fp8:
+        if kv_scale is None:
+            raise ValueError("an fp8 kv_cache needs kv_scale (its dequantisation scales)")
+        kv_cache = kv_cache.view(torch.uint8)
+        page = kv_cache.shape[1]
+        if page % 32 or page & (page - 1):
+            raise NotImplementedError("mla_decode_shared needs an fp8 cache's pages to be a power of two of at least "
+                                      "32 tokens")
+        if torch.is_tensor(kv_scale) and kv_scale.dim() == 2 and kv_scale.numel() > 1:
+            raise NotImplementedError("mla_decode_shared takes one scale per page or per cache, not per token")
+    else:
+        assert kv_scale is None, "kv_scale applies to an fp8 (float8_e4m3fn) kv_cache only"
+        assert q.dtype == kv_cache.dtype
     if q.device.type != "cuda" or kv_cache.device != q.device:
         raise RuntimeError("triton_mla.mla_decode_shared runs on the GPU only: q and kv_cache must be "
                            "on the same HIP device")
@@ -117,8 +130,12 @@ def mla_decode_shared(
             raise ValueError("kv_cache holds no tokens")
         if not _k._aligned(q):
             q = q.clone(memory_format=torch.contiguous_format)
-        if not _k._aligned(kv_cache):
+        if not _k._aligned(kv_cache, 16 if fp8 else 8):
             kv_cache = kv_cache.clone(memory_format=torch.contiguous_format)
+        scale_ptr, scale_stride = None, 0
+        if fp8:
+            kv_scale, scale_stride, _ = _k._scale_layout(kv_scale, kv_cache.shape[0], kv_cache.shape[1], device)
+            scale_ptr = kv_scale.data_ptr()
         lib = _native.load_gil_held()  # the stream's workspace is shared by its calls
         workers = _k._num_sms(device)
         call = _k._CallShape()
@@ -131,7 +148,7 @@ def mla_decode_shared(
             ws, ws_ptr = _k._workspace(call, stream)
             _native.check(lib.tmla_mla_decode_shared(
                 q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1),
-                kv_cache.shape[0], kv_cache.shape[1], block_table.data_ptr(), block_table.stride(0),
+                kv_cache.shape[0], kv_cache.shape[1], scale_ptr, scale_stride, block_table.data_ptr(), block_table.stride(0),
                 block_table.shape[1], cache_seqlens.data_ptr(), prefix_ptr, prefix_len, starts_ptr, groups, batch,
                 q_len, num_heads, head_dim_v, d_rope, _native.DTYPE_CODE[q.dtype], float(softmax_scale), workers,
                 out.data_ptr(), out.stride(0), out.stride(-2), None if lse is None else lse.data_ptr(), ws_ptr,
