@@ -38,13 +38,25 @@ struct SharedItem {
   int32_t pos;
   int32_t first_worker, pieces;
   int32_t mid_row;
-  int32_t pad[5];
+  int32_t index;          // of this item
+  int32_t pad[4];
 };
-static_assert(sizeof(SharedItem) == 64, "one cache line's half per item");
+static_assert(sizeof(SharedItem) == kSharedItemBytes, "the workspace's items");
 struct SharedHeader {
-  int32_t items, prefix_items;  // prefixes first, then the sequences' own tokens
-  int32_t chunk, total;         // positions per worker, and in all
+  int32_t items;
+  int32_t chunk, total;  // positions per worker, and in all
 };
+// Where the partials of one block of up to 128 rows of a sequence lie: row h of
+// the block has pieces[k] partials of its prefix, at row[k] + h + j * rows[k]
+// (k = 0 below `split`, 1 from there on: the block may lie across two prefix
+// items), and own_pieces of its sequence's own tokens.
+struct SharedMerge {
+  int32_t row[2], rows[2], pieces[2];
+  int32_t split;
+  int32_t own_row, own_rows, own_pieces;
+  int32_t pad[2];
+};
+static_assert(sizeof(SharedMerge) == kSharedMergeBytes, "the workspace's merges");
 constexpr int kSharedRows = 128;
 
 struct PartialArgs {
@@ -93,7 +105,7 @@ struct PartialArgs {
 struct SharedArgs : PartialArgs {
   const SharedHeader* header;
   const SharedItem* items;
-  const int32_t* worker_item;
+  const SharedItem* worker_first;  // [workers] the item that each range begins in
 };
 
 // ---------------------------------------------------------------------------
@@ -461,28 +473,31 @@ __device__ __forceinline__ void sequence_slots(const Lens& len_of, int batch, in
 
 // A worker's way along the items of a SharedArgs call.
 struct SharedWalk {
-  int next, items;  // next item, and their number
-  int lo, hi;       // the worker's positions
+  const SharedItem* next;
+  int at, items;  // index of the item after the current one, and their number
+  int lo, hi;     // the worker's positions
 };
 __device__ __forceinline__ bool shared_begin(const SharedArgs& a, int worker, SharedWalk& w) {
   const SharedHeader h = *a.header;
+  w.at = 0;  // (the first item tells)
   w.items = __builtin_amdgcn_readfirstlane(h.items);
   w.lo = __builtin_amdgcn_readfirstlane(worker * h.chunk);
   w.hi = __builtin_amdgcn_readfirstlane(min(w.lo + h.chunk, h.total));
-  if (w.lo >= w.hi) return false;
-  w.next = __builtin_amdgcn_readfirstlane(a.worker_item[worker]);
-  return true;
+  w.next = a.worker_first + worker;
+  return w.lo < w.hi;
 }
 // The next item that has tiles in the worker's range: those tiles, counted
 // from the start of its sequence, the sequence and its tokens. False at the
-// range's end.
+// range's end. The first item comes with the worker's own record, one memory
+// round trip after the kernel's start.
 __device__ __forceinline__ bool shared_next(const SharedArgs& a, SharedWalk& w, SharedItem& item, int& b, int& n_b,
                                             int& t_start, int& t_end) {
-  while (w.next < w.items) {
-    const SharedItem* it = a.items + w.next++;
+  while (w.at < w.items) {
+    const SharedItem* it = w.next;
     const int pos = __builtin_amdgcn_readfirstlane(it->pos);
     const int tiles = __builtin_amdgcn_readfirstlane(it->tiles);
     const int tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
+    w.at = __builtin_amdgcn_readfirstlane(it->index) + 1;
     item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
     item.rows = __builtin_amdgcn_readfirstlane(it->rows);
     item.causal = __builtin_amdgcn_readfirstlane(it->causal);
@@ -490,6 +505,7 @@ __device__ __forceinline__ bool shared_next(const SharedArgs& a, SharedWalk& w, 
     item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
     n_b = __builtin_amdgcn_readfirstlane(it->len);
     b = __builtin_amdgcn_readfirstlane(it->seq);
+    w.next = a.items + w.at;
     if (tiles == 0) continue;
     if (pos - kSegCostTiles >= w.hi) return false;
     t_start = max(w.lo - pos, 0);

@@ -357,7 +357,9 @@ inline int check_generic(const GenericCall& c, const void* workspace, size_t ws_
 // ---------------------------------------------------------------------------
 constexpr int kSharedMaxGroups = 4096;  // what the plan kernel's LDS holds
 constexpr int kSharedMaxWorkers = 65535;
-constexpr int32_t kSharedItemBytes = 64;
+constexpr int32_t kSharedItemBytes = 64, kSharedMergeBytes = 48;
+// Calls of at most so many sequences (and groups) and items are planned in LDS
+constexpr int kSharedSmallBatch = 256, kSharedSmallItems = 512;
 
 struct SharedCall {
   int32_t batch, q_len, heads, groups, workers, dv, dr, dtype, page_size, bt_cols;
@@ -377,7 +379,7 @@ inline int64_t shared_own_items(int64_t batch, int64_t rows) { return batch * ((
 // item's rows; there are at most workers + items pieces, those of a
 // sequence's own tokens of at most min(rows, 128) rows.
 struct SharedWs {
-  size_t items, worker_item, seq_info, mid_lse, mid_o;
+  size_t items, merges, worker_first, mid_lse, mid_o;
   size_t total;  // 0: invalid or too large
 };
 inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t workers) {
@@ -389,9 +391,9 @@ inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t w
   if (mid > INT32_MAX) return w;  // row numbers are 32 bits
   auto al = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   w.items = 256;
-  w.worker_item = w.items + (size_t)al((np + ns) * kSharedItemBytes);
-  w.seq_info = w.worker_item + (size_t)al((int64_t)workers * 4);
-  w.mid_lse = w.seq_info + (size_t)al((int64_t)batch * 8);
+  w.worker_first = w.items + (size_t)al((np + ns) * kSharedItemBytes);
+  w.merges = w.worker_first + (size_t)al((int64_t)workers * kSharedItemBytes);
+  w.mid_lse = w.merges + (size_t)al(ns * kSharedMergeBytes);
   w.mid_o = w.mid_lse + (size_t)al(mid * 4);
   w.total = w.mid_o + (size_t)(mid * 1024);
   return w;
