@@ -12,12 +12,13 @@
 // reads the old rows while it writes the new ones); the cache is written in
 // place.
 //
-// Ranks. The k-th free page is found without a pass of one workgroup over the
-// pool: the first launch counts the free pages of each of up to 1,024 chunks
-// while it copies the counts, and a later launch's workgroup of chunk c
-// sums the counts before c (one load per thread) and ranks its own pages. What
-// bounds the operations is launches and memory round trips where little is
-// copied, and the copies' bytes (each page read and written once) where much is.
+// Ranks. In a large pool the k-th free page is found without a pass of one
+// workgroup over it: the first launch counts the free pages of each chunk
+// while it copies the counts, and a later launch's workgroup of chunk c sums
+// the counts before c and ranks its own pages. A small table and pool are done
+// by one workgroup in LDS instead (pages_small_kernel). What bounds the
+// operations is launches and memory round trips where little is copied, and
+// the copies' bytes (each page read and written once) where much is.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -37,7 +38,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kCopyUnits = 4;       // units per thread and part of a page
 constexpr int kFusedPairs = 256;    // copy: pairs that one launch checks and copies
 constexpr int kMarkThreads = 1024;
-constexpr int kCopyGrid = 4096;     // workgroups of a copy, at most
+constexpr int kCopyGrid = 8192;     // workgroups of a copy, at most
 
 // Pages in units of `unit` bytes (16, 4, 2 or 1: what strides and alignment
 // allow); strides in bytes.
@@ -51,6 +52,10 @@ struct Pool {
   int32_t sc_cols;
 };
 
+// Loads that leave nothing in the caches, and ordinary stores: 4,096 pages of
+// 73,728 bytes (604 MB read and written) in 100 us, 6.0 TB/s; 122 us with
+// ordinary loads, 125 with both non-temporal, 102 to 151 with the stores alone.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <class U>
 __device__ __forceinline__ void copy_part_t(const Pool& p, int src, int dst, int part) {
   const char* s = p.kv + (int64_t)src * p.s0;
@@ -68,7 +73,7 @@ __device__ __forceinline__ void copy_part_t(const Pool& p, int src, int dst, int
       const int r = u / p.row_units;
       off[i] = r * p.s1 + (int64_t)(u - r * p.row_units) * sizeof(U);
     }
-    v[i] = *reinterpret_cast<const U*>(s + off[i]);
+    v[i] = __builtin_nontemporal_load(reinterpret_cast<const U*>(s + off[i]));
   }
 #pragma unroll
   for (int i = 0; i < kCopyUnits; ++i)
@@ -78,7 +83,7 @@ __device__ __forceinline__ void copy_part_t(const Pool& p, int src, int dst, int
 // One part of page src to page dst, and with part 0 its scales. The pages
 // differ.
 __device__ __forceinline__ void copy_part(const Pool& p, int src, int dst, int part) {
-  if (p.unit == 16) copy_part_t<uint4>(p, src, dst, part);
+  if (p.unit == 16) copy_part_t<u32x4>(p, src, dst, part);
   else if (p.unit == 4) copy_part_t<uint32_t>(p, src, dst, part);
   else if (p.unit == 2) copy_part_t<uint16_t>(p, src, dst, part);
   else copy_part_t<uint8_t>(p, src, dst, part);
@@ -86,6 +91,27 @@ __device__ __forceinline__ void copy_part(const Pool& p, int src, int dst, int p
     for (int j = threadIdx.x; j < p.sc_cols; j += kThreads)
       *reinterpret_cast<float*>(p.scale + (int64_t)dst * p.sc0 + j * p.sc1) =
           *reinterpret_cast<const float*>(p.scale + (int64_t)src * p.sc0 + j * p.sc1);
+}
+
+// Four consecutive values of an array of n, on any boundary (0 past its end).
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4a __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ i32x4a load4(const int32_t* a, int i, int n) {
+  if (i + 4 <= n) return *reinterpret_cast<const i32x4a*>(a + i);
+  i32x4a v = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i + k < n) v[k] = a[i + k];
+  return v;
+}
+__device__ __forceinline__ void store4(int32_t* a, int i, int n, i32x4a v) {
+  if (i + 4 <= n) {
+    *reinterpret_cast<i32x4a*>(a + i) = v;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i + k < n) a[i + k] = v[k];
 }
 
 __device__ __forceinline__ bool held(int e, int pages) { return e >= 0 && e < pages; }
@@ -135,27 +161,38 @@ __device__ __forceinline__ int block_before(int x, int* sums, int& total) {
 // is not written.
 
 // Up to kFusedPairs pairs: every workgroup checks the pair it copies against
-// all of them; the last workgroup counts the refused ones.
+// all of them; the first one counts the refused pairs.
 __global__ __launch_bounds__(kThreads) void pages_copy_few_kernel(Pool p, const int32_t* src, const int32_t* dst, int n,
                                                                   int32_t* refused) {
-  __shared__ int s_src[kFusedPairs], s_dst[kFusedPairs], s_sums[kWaves], s_last;
+  __shared__ int s_src[kFusedPairs];
+  __shared__ __attribute__((aligned(16))) int s_dst[kFusedPairs];
+  __shared__ int s_sums[kWaves], s_last;
   const int tid = threadIdx.x;
   bool valid = false;  // of pair tid; others can have no page in common with a valid pair
-  if (tid < n) {
-    const int a = src[tid], b = dst[tid];
-    valid = held(a, p.pages) && held(b, p.pages);
+  {
+    int a = -1, b = -1;
+    if (tid < n) {
+      a = src[tid];
+      b = dst[tid];
+      valid = held(a, p.pages) && held(b, p.pages);
+    }
     s_src[tid] = valid ? a : -1;
     s_dst[tid] = valid ? b : -1;
   }
   if (tid == 0) s_last = -1;
   __syncthreads();
-  if ((int)blockIdx.x == (int)gridDim.x - 1) {
+  if (blockIdx.x == 0) {
     bool bad = tid < n && !valid;
     if (valid) {
+      const int a = s_src[tid], b = s_dst[tid];
       int writer = -1;  // last pair that writes the source
-      for (int j = 0; j < n; ++j) {
-        if (j > tid && s_dst[j] == s_dst[tid]) bad = true;
-        if (s_dst[j] == s_src[tid]) writer = j;
+      for (int j = 0; j < n; j += 4) {
+        const i32x4 d = *reinterpret_cast<const i32x4*>(s_dst + j);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          bad |= j + k > tid && d[k] == b;
+          writer = d[k] == a ? j + k : writer;
+        }
       }
       bad |= writer >= 0 && s_src[writer] != s_dst[writer];
     }
@@ -163,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void pages_copy_few_kernel(Pool p, const 
     if (tid == 0) *refused = t;
     return;
   }
-  const int i = blockIdx.x / p.parts, part = blockIdx.x - i * p.parts;
+  const int i = (blockIdx.x - 1) / p.parts, part = blockIdx.x - 1 - i * p.parts;
   const int a = s_src[i], b = s_dst[i];
   if (a < 0 || a == b) return;
   if (valid && s_dst[tid] == a) atomicMax(&s_last, tid);
@@ -172,33 +209,86 @@ __global__ __launch_bounds__(kThreads) void pages_copy_few_kernel(Pool p, const 
   copy_part(p, a, b, part);
 }
 
-// More pairs: one workgroup marks each destination with the last pair that
-// writes it (mark[page] counts only if that pair's destination is the page:
-// the other pages' marks are never initialised) and lists what is to be
-// copied.
+// More pairs: one workgroup checks them and lists what is to be copied. It
+// sets the destinations' bits in LDS (of pools of up to kMarkBits pages): where
+// no bit is met twice, no source has one, every id is in the pool and no page
+// goes to itself, all pairs copy. Otherwise it marks each destination with the last pair that
+// writes it; mark[page] counts only if that pair's destination is the page, as
+// the other pages' marks are never initialised. (Atomics of the workgroup's
+// scope: a fence for the whole device would write the L2 back.) 4,096 pairs:
+// MARK_US us, 28 when every call marked the pool's memory.
+constexpr int kMarkBits = 1 << 20;
+
 __global__ __launch_bounds__(kMarkThreads) void pages_mark_kernel(const int32_t* src, const int32_t* dst, int n,
                                                                   int pages, int32_t* mark, int2* list,
                                                                   int32_t* refused) {
+  __shared__ unsigned s_bits[kMarkBits / 32];
   __shared__ int s_refused;
-  if (threadIdx.x == 0) s_refused = 0;
-  auto valid = [&](int i) { return held(src[i], pages) && held(dst[i], pages); };
-  for (int i = threadIdx.x; i < n; i += kMarkThreads)
-    if (valid(i)) mark[dst[i]] = -1;
-  __threadfence();  // the marks are in place before another wave's atomics
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kMarkThreads)
-    if (valid(i)) atomicMax(&mark[dst[i]], i);
-  __threadfence();
-  __syncthreads();
+  constexpr int T = kMarkThreads, PER = 4;
+  const int tid = threadIdx.x;
+  auto valid = [&](int a, int b) { return held(a, pages) && held(b, pages); };
+  if (pages <= kMarkBits) {
+    int a[PER], b[PER];  // the first pairs of this thread
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = tid + k * T;
+      a[k] = i < n ? src[i] : -1;
+      b[k] = i < n ? dst[i] : -1;
+    }
+    for (int w = tid; w < (pages + 31) / 32; w += T) s_bits[w] = 0;
+    __syncthreads();
+    bool bad = false;
+    auto set = [&](int x, int y) {
+      if (!valid(x, y) || x == y) bad = true;
+      else bad |= (atomicOr(&s_bits[y / 32], 1u << (y % 32)) >> (y % 32)) & 1;
+    };
+    auto test = [&](int x) { bad |= held(x, pages) && (s_bits[x / 32] >> (x % 32) & 1); };
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (tid + k * T < n) set(a[k], b[k]);
+    for (int i = tid + PER * T; i < n; i += T) set(src[i], dst[i]);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) test(a[k]);
+    for (int i = tid + PER * T; i < n; i += T) test(src[i]);
+    if (!__syncthreads_or(bad)) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (tid + k * T < n) list[tid + k * T] = make_int2(a[k], b[k]);
+      for (int i = tid + PER * T; i < n; i += T) list[i] = make_int2(src[i], dst[i]);
+      if (tid == 0) *refused = 0;
+      return;
+    }
+  }
+  if (tid == 0) s_refused = 0;
+  auto store = [&](int page, int v) {
+    __hip_atomic_store(&mark[page], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  auto load = [&](int page) {
+    return __hip_atomic_load(&mark[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  // this wave's memory operations are done before the others go on
+  auto barrier = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  for (int i = tid; i < n; i += T)
+    if (valid(src[i], dst[i])) store(dst[i], -1);
+  barrier();
+  for (int i = tid; i < n; i += T)
+    if (valid(src[i], dst[i]))
+      __hip_atomic_fetch_max(&mark[dst[i]], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  barrier();
   int bad = 0;
-  for (int i = threadIdx.x; i < n; i += kMarkThreads) {
+  for (int i = tid; i < n; i += T) {
     const int a = src[i], b = dst[i];
-    bool ok = valid(i);
+    bool ok = valid(a, b);
     if (ok) {
-      ok = __hip_atomic_load(&mark[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
-      if (ok && a != b) {
-        const int m = __hip_atomic_load(&mark[a], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (m >= 0 && m < n && valid(m) && dst[m] == a && src[m] != a) ok = false;
+      ok = load(b) == i;
+      const int m = load(a);
+      if (a != b && m >= 0 && m < n) {
+        const int ma = src[m], mb = dst[m];
+        if (valid(ma, mb) && mb == a && ma != a) ok = false;
       }
     }
     bad += !ok;
@@ -206,11 +296,12 @@ __global__ __launch_bounds__(kMarkThreads) void pages_mark_kernel(const int32_t*
   }
   if (bad) atomicAdd(&s_refused, bad);
   __syncthreads();
-  if (threadIdx.x == 0) *refused = s_refused;
+  if (tid == 0) *refused = s_refused;
 }
 
-__global__ __launch_bounds__(kThreads) void pages_copy_kernel(Pool p, const int2* list, int n) {
-  const int64_t total = (int64_t)n * p.parts;
+// count: the pairs listed, if the host does not know.
+__global__ __launch_bounds__(kThreads) void pages_copy_kernel(Pool p, const int2* list, int n, const int32_t* count) {
+  const int64_t total = (int64_t)(count ? min(n, *count) : n) * p.parts;
   for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
     const int i = (int)(w / p.parts), part = (int)(w - (int64_t)i * p.parts);
     const int2 pair = list[i];
@@ -253,10 +344,11 @@ template <bool USED>
 __device__ __forceinline__ void count_chunk(const Tables& t, int c, int* sums) {
   const int lo = c * t.chunk, hi = min(lo + t.chunk, t.pages);
   int n = 0;
-  for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
-    const int r = t.refs[i];
-    if (t.new_refs) t.new_refs[i] = r;
-    n += USED ? r > 0 : r <= 0;
+  for (int i = lo + 4 * threadIdx.x; i < hi; i += 4 * kThreads) {
+    const i32x4a r = load4(t.refs, i, hi);
+    if (t.new_refs) store4(t.new_refs, i, hi, r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += i + k < hi && (USED ? r[k] > 0 : r[k] <= 0);
   }
   n = block_total(n, sums);
   if (threadIdx.x == 0) t.chunk_count[c] = n;
@@ -315,24 +407,35 @@ __global__ __launch_bounds__(kThreads) void pages_fork_kernel(Tables t) {
 // fork and free, second launch: the counts of rows that nobody continues and of
 // rows that share another's pages. A page's count passes zero as often up as
 // down, whatever the order, so the chunk's free pages come out right too.
-__device__ __forceinline__ void add_ref(const Tables& t, int e, int d) {
-  const int old = atomicAdd(&t.new_refs[e], d);
-  const int was = old <= 0, is = old + d <= 0;
-  if (t.chunk_count && was != is) atomicAdd(&t.chunk_count[e / t.chunk], is - was);
-}
-
+// (The chunks' sums meet in LDS first: 3,000 atomics on three addresses took
+// 20 us of a kernel of 24.)
 __global__ __launch_bounds__(kThreads) void pages_fork_refs_kernel(Tables t) {
+  __shared__ int s_free[kPagesMaxChunks];
   const int i = blockIdx.x, tid = threadIdx.x;
-  if (!t.has_child[i]) {
+  const bool release = !t.has_child[i], share = t.source[i] != -2;
+  if (!release && !share) return;
+  if (t.chunk_count)
+    for (int c = tid; c < t.chunks; c += kThreads) s_free[c] = 0;
+  __syncthreads();
+  auto add = [&](int e, int d) {
+    const int old = atomicAdd(&t.new_refs[e], d);
+    const int was = old <= 0, is = old + d <= 0;
+    if (t.chunk_count && was != is) atomicAdd(&s_free[e / t.chunk], is - was);
+  };
+  if (release) {
     const int32_t* row = t.table + (int64_t)i * t.table_s;
     for (int j = tid; j < t.width; j += kThreads)
-      if (held(row[j], t.pages)) add_ref(t, row[j], -1);
+      if (held(row[j], t.pages)) add(row[j], -1);
   }
-  if (t.source[i] != -2) {
+  if (share) {
     const int32_t* row = t.new_table + (int64_t)i * t.width;
     for (int j = tid; j < t.width; j += kThreads)
-      if (row[j] >= 0) add_ref(t, row[j], 1);
+      if (row[j] >= 0) add(row[j], 1);
   }
+  if (!t.chunk_count) return;
+  __syncthreads();
+  for (int c = tid; c < t.chunks; c += kThreads)
+    if (s_free[c]) atomicAdd(&t.chunk_count[c], s_free[c]);
 }
 
 // The pages taken (fork and reserve): workgroup c ranks the free pages of chunk
@@ -353,15 +456,22 @@ __global__ __launch_bounds__(kThreads) void pages_take_kernel(Tables t) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *t.missing = (int32_t)min(missing, (int64_t)INT32_MAX);
   if (missing > 0 || before >= want) return;
   const int lo = blockIdx.x * t.chunk, hi = min(lo + t.chunk, t.pages);
-  for (int i0 = lo; i0 < hi && before < want; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const bool f = i < hi && t.new_refs[i] <= 0;
-    int n;
-    const int rank = before + block_before(f, sums, n);
-    if (f && rank < want) {
-      t.ids[rank] = i;
-      t.new_refs[i] = 1;
-    }
+  for (int i0 = lo; i0 < hi && before < want; i0 += 4 * kThreads) {
+    const int i = i0 + 4 * threadIdx.x;
+    const i32x4a r = load4(t.new_refs, i, hi);
+    int f = 0, n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f += i + k < hi && r[k] <= 0;
+    int rank = before + block_before(f, sums, n);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < hi && r[k] <= 0) {
+        if (rank < want) {
+          t.ids[rank] = i + k;
+          t.new_refs[i + k] = 1;
+        }
+        ++rank;
+      }
     before += n;
   }
 }
@@ -371,7 +481,10 @@ __global__ __launch_bounds__(kThreads) void pages_take_kernel(Tables t) {
 __global__ __launch_bounds__(kThreads) void pages_fork_copy_kernel(Tables t, Pool p) {
   __shared__ int sums[kWaves];
   const int i = blockIdx.x / p.parts, part = blockIdx.x - i * p.parts, tid = threadIdx.x;
-  if (*t.missing > 0) {
+  const int missing = *t.missing, src = t.source[i], at = t.new_seqlens[i] / t.page_size;
+  int before = 0;  // pages given to the rows before
+  for (int j = tid; j < i; j += kThreads) before += t.need[j];
+  if (missing > 0) {
     if (part == 0) {
       for (int j = tid; j < t.width; j += kThreads)
         t.new_table[(int64_t)i * t.width + j] = t.table[(int64_t)i * t.table_s + j];
@@ -381,13 +494,10 @@ __global__ __launch_bounds__(kThreads) void pages_fork_copy_kernel(Tables t, Poo
       t.new_refs[j] = t.refs[j];
     return;
   }
-  const int src = t.source[i];
   if (src < 0) return;
-  int all, rank;
-  sums_of(t.need, i, i, sums, all, rank);
-  const int dst = t.ids[rank];
+  const int dst = t.ids[block_total(before, sums)];
   copy_part(p, src, dst, part);
-  if (part == 0 && tid == 0) t.new_table[(int64_t)i * t.width + t.seqlens[t.parents[i]] / t.page_size] = dst;
+  if (part == 0 && tid == 0) t.new_table[(int64_t)i * t.width + at] = dst;
 }
 
 // free, first launch
@@ -441,9 +551,11 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_kernel(Tables t) {
 __global__ __launch_bounds__(kThreads) void pages_reserve_fill_kernel(Tables t) {
   __shared__ int sums[kWaves];
   const int i = blockIdx.x;
-  if (*t.missing > 0 || t.need[i] == 0) return;
-  int all, rank;
-  sums_of(t.need, i, i, sums, all, rank);
+  const int missing = *t.missing, mine = t.need[i];
+  int rank = 0;
+  for (int j = threadIdx.x; j < i; j += kThreads) rank += t.need[j];
+  if (missing > 0 || mine == 0) return;
+  rank = block_total(rank, sums);
   const int want = min(pages_needed(t, i), t.width);
   int32_t* row = t.new_table + (int64_t)i * t.width;
   for (int j0 = 0; j0 < want; j0 += kThreads) {
@@ -453,6 +565,183 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_fill_kernel(Tables t) 
     const int r = rank + block_before(lack, sums, n);
     if (lack) row[j] = t.ids[r];
     rank += n;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Fork, free or reserve by one workgroup, the counts and the rows' values in
+// LDS: tables of at most kPagesSmallEntries entries and pools of at most
+// kPagesSmallPages pages. One launch (and the copies') instead of three or
+// four: SMALL_US.
+// ---------------------------------------------------------------------------
+enum class Op { kFork, kFree, kReserve };
+constexpr int kSmallThreads = 1024;
+
+template <Op OP>
+__global__ __launch_bounds__(kSmallThreads) void pages_small_kernel(Tables t, int2* list, int32_t* listed) {
+  constexpr int T = kSmallThreads;
+  __shared__ int s_refs[kPagesSmallPages];
+  __shared__ int s_len[kPagesSmallRows];     // length of the row's parent (reserve: entries it should hold)
+  __shared__ int s_parent[kPagesSmallRows];  // -1: the row ends empty
+  __shared__ int s_first[kPagesSmallRows];   // lowest child of the row
+  __shared__ int s_need[kPagesSmallRows], s_rank[kPagesSmallRows];
+  __shared__ int s_src[kPagesSmallRows];
+  __shared__ int s_ids[kPagesSmallPages];
+  __shared__ int s_sums[T / 64];
+  __shared__ long long s_beyond;
+  const int tid = threadIdx.x, B = t.batch, W = t.width, entries = B * W;
+  auto before_of = [&](int x, int& total) {  // scan over the workgroup
+    const int incl = wave_scan(x);
+    __syncthreads();
+    if ((tid & 63) == 63) s_sums[tid >> 6] = incl;
+    __syncthreads();
+    int head = 0;
+    total = 0;
+    for (int w = 0; w < T / 64; ++w) {
+      const int v = s_sums[w];
+      if (w < (tid >> 6)) head += v;
+      total += v;
+    }
+    return head + incl - x;
+  };
+  if (tid == 0) s_beyond = 0;
+  for (int i = 4 * tid; i < t.pages; i += 4 * T) {
+    const i32x4a r = load4(t.refs, i, t.pages);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < t.pages) s_refs[i + k] = r[k];
+  }
+  for (int i = tid; i < B; i += T) {
+    s_first[i] = INT32_MAX;
+    s_need[i] = 0;
+    s_src[i] = -1;
+    if constexpr (OP == Op::kFork) {
+      const int p = t.parents[i];
+      s_parent[i] = p >= 0 && p < B ? p : -1;
+    } else if constexpr (OP == Op::kFree) {
+      s_parent[i] = t.ended[i] ? -1 : i;
+    } else {
+      const int want = pages_needed(t, i);
+      s_len[i] = min(want, W);
+      if (want > W) atomicAdd(reinterpret_cast<unsigned long long*>(&s_beyond), (unsigned long long)(want - W));
+    }
+  }
+  __syncthreads();
+  if constexpr (OP != Op::kReserve) {
+    for (int i = tid; i < B; i += T) {
+      const int p = s_parent[i], n = p >= 0 ? t.seqlens[p] : 0;
+      s_len[i] = n;
+      t.new_seqlens[i] = n;
+      if (p >= 0) atomicMin(&s_first[p], i);
+    }
+    __syncthreads();
+  }
+  // the rows, but for the pages they will be given
+  for (int x = tid; x < entries; x += T) {
+    const int i = x / W, j = x - i * W;
+    if constexpr (OP == Op::kReserve) {
+      const int e = t.table[(int64_t)i * t.table_s + j];
+      t.new_table[x] = e;
+      if (j < s_len[i] && !held(e, t.pages)) atomicAdd(&s_need[i], 1);
+    } else {
+      const int p = s_parent[i];
+      int e = -1;
+      if (p >= 0) {
+        const int old = t.table[(int64_t)p * t.table_s + j];
+        const bool keeper = s_first[p] == i;
+        if constexpr (OP == Op::kFree) {
+          e = old;
+        } else if (held(old, t.pages)) {
+          const int n = s_len[i], full = n > 0 ? n / t.page_size : 0;
+          if (keeper || j < full) {
+            e = old;
+            if (!keeper) atomicAdd(&s_refs[e], 1);
+          } else if (j == full && n > 0 && n % t.page_size) {
+            s_src[i] = old;
+            s_need[i] = 1;
+          }
+        }
+      }
+      t.new_table[x] = e;
+      if (s_first[i] == INT32_MAX) {  // nobody continues row i
+        const int own = t.table[(int64_t)i * t.table_s + j];
+        if (held(own, t.pages)) atomicSub(&s_refs[own], 1);
+      }
+    }
+  }
+  __syncthreads();
+  int want = 0, missing = 0;
+  if constexpr (OP != Op::kFree) {
+    for (int i0 = 0; i0 < B; i0 += T) {
+      const int i = i0 + tid;
+      int n;
+      const int at = before_of(i < B ? s_need[i] : 0, n) + want;
+      if (i < B) s_rank[i] = at;
+      want += n;
+    }
+    // the lowest `want` free pages
+    int found = 0;
+    for (int i0 = 0; i0 < t.pages && found < want; i0 += 4 * T) {
+      const int i = i0 + 4 * tid;
+      int f = 0, n;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f += i + k < t.pages && s_refs[min(i + k, t.pages - 1)] <= 0;
+      int rank = before_of(f, n) + found;
+      if (f)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k < t.pages && s_refs[i + k] <= 0) {
+            if (rank < want) s_ids[rank] = i + k;
+            ++rank;
+          }
+      found += n;
+    }
+    const int64_t lack = max(want - found, 0) + s_beyond;
+    missing = (int)min(lack, (int64_t)INT32_MAX);
+    if (tid == 0) *t.missing = missing;
+    __syncthreads();
+  }
+  if (missing > 0) {  // everything as it was
+    for (int x = tid; x < entries; x += T) t.new_table[x] = t.table[(int64_t)(x / W) * t.table_s + x % W];
+    for (int i = tid; i < t.pages; i += T) t.new_refs[i] = t.refs[i];
+    if constexpr (OP == Op::kFork) {
+      for (int i = tid; i < B; i += T) t.new_seqlens[i] = t.seqlens[i];
+      if (tid == 0) *listed = 0;
+    }
+    return;
+  }
+  if constexpr (OP != Op::kFree) {
+    for (int k = tid; k < want; k += T) s_refs[s_ids[k]] = 1;
+    if constexpr (OP == Op::kFork) {
+      for (int i = tid; i < B; i += T)
+        if (s_need[i]) {
+          const int page = s_ids[s_rank[i]];
+          t.new_table[(int64_t)i * W + s_len[i] / t.page_size] = page;
+          list[s_rank[i]] = make_int2(s_src[i], page);
+        }
+      if (tid == 0) *listed = want;
+    } else {
+      // a wave per row, its lacking entries in order
+      const int lane = tid & 63;
+      for (int i = tid >> 6; i < B; i += T / 64) {
+        if (s_need[i] == 0) continue;
+        int rank = s_rank[i];
+        for (int j0 = 0; j0 < s_len[i]; j0 += 64) {
+          const int j = j0 + lane;
+          const bool lack = j < s_len[i] && !held(t.table[(int64_t)i * t.table_s + j], t.pages);
+          const uint64_t m = __ballot(lack);
+          if (lack) t.new_table[(int64_t)i * W + j] = s_ids[rank + __popcll(m & ((1ull << lane) - 1))];
+          rank += __popcll(m);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = 4 * tid; i < t.pages; i += 4 * T) {
+    i32x4a r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = s_refs[min(i + k, t.pages - 1)];
+    store4(t.new_refs, i, t.pages, r);
   }
 }
 
@@ -485,22 +774,34 @@ __global__ __launch_bounds__(kThreads) void pages_rank_kernel(Tables t, int32_t*
     t.missing[0] = L - stay;  // pages that move
   }
   const int lo = blockIdx.x * t.chunk, hi = min(lo + t.chunk, t.pages);
-  for (int i0 = lo; i0 < hi; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const int r = i < hi ? t.refs[i] : 0;
-    const bool u = r > 0;
-    int n;
-    const int b = before + block_before(u, sums, n);  // used pages before page i
-    if (i < hi) {
-      if (i < L) {
-        if (u) t.new_refs[i] = r;
-        else to[i - b] = i;
-      } else {
-        if (u) from[b - stay] = i;
-        rank_of[i] = u ? b - stay : -1;
-        t.new_refs[i] = u ? 0 : r;
+  for (int i0 = lo; i0 < hi; i0 += 4 * kThreads) {
+    const int i = i0 + 4 * threadIdx.x;
+    const i32x4a r = load4(t.refs, i, hi);
+    int u = 0, n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u += i + k < hi && r[k] > 0;
+    int b = before + block_before(u, sums, n);  // used pages before page i + k
+    i32x4a counts = r, ranks;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool used = r[k] > 0;
+      ranks[k] = -1;
+      if (i + k < hi) {
+        if (i + k < L) {
+          if (!used) to[i + k - b] = i + k;
+        } else if (used) {
+          from[b - stay] = i + k;
+          ranks[k] = b - stay;
+          counts[k] = 0;
+        }
       }
+      b += used;
     }
+    store4(rank_of, i, hi, ranks);
+    // (the counts of the free pages among the first L come with their pages)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < hi && !(i + k < L && r[k] <= 0)) t.new_refs[i + k] = counts[k];
     before += n;
   }
 }
@@ -563,6 +864,11 @@ void set_chunks(Tables& t) {
   t.chunks = (t.pages + t.chunk - 1) / t.chunk;
 }
 
+bool is_small(const Tables& t) {
+  return t.batch > 0 && t.batch <= kPagesSmallRows && t.pages <= kPagesSmallPages &&
+         (int64_t)t.batch * t.width <= kPagesSmallEntries;
+}
+
 }  // namespace
 }  // namespace tmla
 
@@ -607,7 +913,7 @@ int tmla_pages_copy(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t 
   TMLA_LAUNCHED("pages_mark_kernel");
   const int64_t total = (int64_t)pairs * p.parts;
   hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)(total < kCopyGrid ? total : kCopyGrid)), dim3(kThreads), 0, s,
-                     p, list, pairs);
+                     p, list, pairs, (const int32_t*)nullptr);
   TMLA_LAUNCHED("pages_copy_kernel");
   return TMLA_OK;
 }
@@ -650,6 +956,17 @@ int tmla_pages_fork(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t 
   t.ids = reinterpret_cast<int32_t*>(ws + w.ids);
   t.missing = missing;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (is_small(t)) {
+    int2* list = reinterpret_cast<int2*>(ws + w.ids2);
+    int32_t* listed = reinterpret_cast<int32_t*>(ws + w.flag);
+    hipLaunchKernelGGL(pages_small_kernel<Op::kFork>, dim3(1), dim3(kSmallThreads), 0, s, t, list, listed);
+    TMLA_LAUNCHED("pages_small_kernel");
+    const int64_t most = (int64_t)batch * p.parts;
+    hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)(most < kCopyGrid ? most : kCopyGrid)), dim3(kThreads), 0, s, p,
+                       list, batch, listed);
+    TMLA_LAUNCHED("pages_copy_kernel");
+    return TMLA_OK;
+  }
   hipLaunchKernelGGL(pages_fork_kernel, dim3(t.chunks + batch), dim3(kThreads), 0, s, t);
   TMLA_LAUNCHED("pages_fork_kernel");
   if (batch > 0) {
@@ -694,6 +1011,12 @@ int tmla_pages_free(const int32_t* table, int64_t table_stride, int32_t batch, i
   t.source = t.need + batch;
   t.has_child = t.source + batch;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (is_small(t)) {
+    hipLaunchKernelGGL(pages_small_kernel<Op::kFree>, dim3(1), dim3(kSmallThreads), 0, s, t, (int2*)nullptr,
+                       (int32_t*)nullptr);
+    TMLA_LAUNCHED("pages_small_kernel");
+    return TMLA_OK;
+  }
   hipLaunchKernelGGL(pages_free_kernel, dim3(t.chunks + batch), dim3(kThreads), 0, s, t);
   TMLA_LAUNCHED("pages_free_kernel");
   if (batch > 0) {
@@ -735,6 +1058,12 @@ int tmla_pages_reserve(const int32_t* table, int64_t table_stride, int32_t batch
   t.ids = reinterpret_cast<int32_t*>(ws + w.ids);
   t.missing = missing;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (is_small(t)) {
+    hipLaunchKernelGGL(pages_small_kernel<Op::kReserve>, dim3(1), dim3(kSmallThreads), 0, s, t, (int2*)nullptr,
+                       (int32_t*)nullptr);
+    TMLA_LAUNCHED("pages_small_kernel");
+    return TMLA_OK;
+  }
   hipLaunchKernelGGL(pages_reserve_kernel, dim3(t.chunks + batch), dim3(kThreads), 0, s, t);
   TMLA_LAUNCHED("pages_reserve_kernel");
   hipLaunchKernelGGL(pages_take_kernel, dim3(t.chunks), dim3(kThreads), 0, s, t);

@@ -436,14 +436,16 @@ inline int check_shared(const SharedCall& c, const void* workspace, size_t ws_by
 // ---------------------------------------------------------------------------
 // Page operations (cache_pages.hip)
 // ---------------------------------------------------------------------------
-constexpr int kPagesMaxChunks = 1024;
+constexpr int kPagesMaxChunks = 4096;
+// Tables and pools that one workgroup does in LDS
+constexpr int kPagesSmallRows = 1024, kPagesSmallPages = 12288, kPagesSmallEntries = 1 << 13;
 constexpr int32_t kPagesMaxRows = 1 << 20;  // rows of a table
 
-// Pages per chunk of the counts: at most 1,024 chunks of at least 4,096 pages
-// (below, one chunk's pages take one workgroup less than a launch).
+// Pages per chunk of the counts: at most 4,096 chunks of at least 1,024 pages,
+// one turn of a workgroup of 256 threads with four pages each.
 inline int32_t pages_chunk(int32_t pages) {
   const int64_t per = ((int64_t)pages + kPagesMaxChunks - 1) / kPagesMaxChunks;
-  return per < 4096 ? 4096 : (int32_t)per;
+  return (int32_t)(per < 1024 ? 1024 : (per + 1023) / 1024 * 1024);
 }
 
 // Largest unit of 16, 4, 2 or 1 bytes that address, strides and row bytes allow.
@@ -490,7 +492,8 @@ inline PagesWs pages_ws(int64_t pages, int32_t batch, int32_t pairs) {
   w.rows = w.chunks + al(kPagesMaxChunks * 4);
   w.ids = w.rows + al((int64_t)batch * 12);
   w.ids2 = w.ids + al(pages * 4);
-  w.ids3 = w.ids2 + al(pages * 4);
+  // (also the pairs that a fork lists)
+  w.ids3 = w.ids2 + al(pages * 4 > (int64_t)batch * 8 ? pages * 4 : (int64_t)batch * 8);
   w.pairs = w.ids3 + al(pages * 4);
   w.total = w.pairs + al((int64_t)pairs * 8);
   return w;
