@@ -98,15 +98,24 @@ struct PartialArgs {
   int64_t sc_s0, sc_s1;    // element strides
 };
 
-// Shared prefixes: the work items and where each worker's range of them
-// begins, as the plan kernel of mla_decode_shared.hip wrote them. num_heads is
-// the rows of a sequence (query tokens x heads). A type of its own: the other
-// kernels' arguments, and so their code, stay as they are.
+// Shared prefixes (mla_decode_shared.hip). num_heads is the rows of a sequence
+// (query tokens x heads). Types of their own: the other kernels' arguments, and
+// so their code, stay as they are.
 struct SharedArgs : PartialArgs {
-  const SharedHeader* header;
-  const SharedItem* items;
-  const SharedItem* worker_first;  // [workers] the item that each range begins in
+  const int32_t* prefix_lens;   // [groups], or null: prefix_len for each
+  const int32_t* group_starts;  // [groups + 1], or null: one group of the whole batch
+  int32_t prefix_len, groups, capacity;
+  SharedMerge* merges;          // [batch, blocks of 128 rows]
+  // as the plan kernel writes them
+  SharedHeader* header;
+  SharedItem* items;
+  SharedItem* worker_first;     // [workers] the item that each range begins in
 };
+// The workers make the plan themselves (shared_plan.h).
+struct SharedFusedArgs : SharedArgs {
+  SharedItem* worker_list;      // [workers, kSharedSmallItems]
+};
+constexpr int kSharedList = 44;  // items that a worker's list holds in LDS
 
 // ---------------------------------------------------------------------------
 // small device helpers
@@ -471,13 +480,38 @@ __device__ __forceinline__ void sequence_slots(const Lens& len_of, int batch, in
   }
 }
 
-// A worker's way along the items of a SharedArgs call.
+// Item *it as a worker with positions [lo, hi) sees it: its tiles in that range,
+// counted from the start of its sequence, the sequence and its tokens. False if
+// it has none there.
+__device__ __forceinline__ bool shared_take(const SharedItem* it, int lo, int hi, SharedItem& item, int& b, int& n_b,
+                                            int& t_start, int& t_end) {
+  const int pos = __builtin_amdgcn_readfirstlane(it->pos);
+  const int tiles = __builtin_amdgcn_readfirstlane(it->tiles);
+  const int tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
+  item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
+  item.rows = __builtin_amdgcn_readfirstlane(it->rows);
+  item.causal = __builtin_amdgcn_readfirstlane(it->causal);
+  item.first_worker = __builtin_amdgcn_readfirstlane(it->first_worker);
+  item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
+  item.index = __builtin_amdgcn_readfirstlane(it->index);
+  n_b = __builtin_amdgcn_readfirstlane(it->len);
+  b = __builtin_amdgcn_readfirstlane(it->seq);
+  t_start = max(lo - pos, 0);
+  t_end = min(tiles, hi - pos);
+  if (t_start >= t_end) return false;  // no tiles, or only positions before its first
+  t_start += tile0;
+  t_end += tile0;
+  return true;
+}
+
+// A worker's way along the items of a SharedArgs call. The first item comes
+// with the worker's own record, one memory round trip after the kernel's start.
 struct SharedWalk {
   const SharedItem* next;
   int at, items;  // index of the item after the current one, and their number
   int lo, hi;     // the worker's positions
 };
-__device__ __forceinline__ bool shared_begin(const SharedArgs& a, int worker, SharedWalk& w) {
+__device__ __forceinline__ bool shared_begin(const SharedArgs& a, int worker, SharedWalk& w, void*, SharedItem*) {
   const SharedHeader h = *a.header;
   w.at = 0;  // (the first item tells)
   w.items = __builtin_amdgcn_readfirstlane(h.items);
@@ -486,34 +520,15 @@ __device__ __forceinline__ bool shared_begin(const SharedArgs& a, int worker, Sh
   w.next = a.worker_first + worker;
   return w.lo < w.hi;
 }
-// The next item that has tiles in the worker's range: those tiles, counted
-// from the start of its sequence, the sequence and its tokens. False at the
-// range's end. The first item comes with the worker's own record, one memory
-// round trip after the kernel's start.
-__device__ __forceinline__ bool shared_next(const SharedArgs& a, SharedWalk& w, SharedItem& item, int& b, int& n_b,
-                                            int& t_start, int& t_end) {
+__device__ __forceinline__ bool shared_next(const SharedArgs& a, int, SharedWalk& w, SharedItem& item, int& b, int& n_b,
+                                            int& t_start, int& t_end, const SharedItem*) {
   while (w.at < w.items) {
     const SharedItem* it = w.next;
-    const int pos = __builtin_amdgcn_readfirstlane(it->pos);
-    const int tiles = __builtin_amdgcn_readfirstlane(it->tiles);
-    const int tile0 = __builtin_amdgcn_readfirstlane(it->tile0);
-    w.at = __builtin_amdgcn_readfirstlane(it->index) + 1;
-    item.row0 = __builtin_amdgcn_readfirstlane(it->row0);
-    item.rows = __builtin_amdgcn_readfirstlane(it->rows);
-    item.causal = __builtin_amdgcn_readfirstlane(it->causal);
-    item.first_worker = __builtin_amdgcn_readfirstlane(it->first_worker);
-    item.mid_row = __builtin_amdgcn_readfirstlane(it->mid_row);
-    n_b = __builtin_amdgcn_readfirstlane(it->len);
-    b = __builtin_amdgcn_readfirstlane(it->seq);
+    if (__builtin_amdgcn_readfirstlane(it->pos) - kSegCostTiles >= w.hi) return false;
+    const bool any = shared_take(it, w.lo, w.hi, item, b, n_b, t_start, t_end);
+    w.at = item.index + 1;
     w.next = a.items + w.at;
-    if (tiles == 0) continue;
-    if (pos - kSegCostTiles >= w.hi) return false;
-    t_start = max(w.lo - pos, 0);
-    t_end = min(tiles, w.hi - pos);
-    if (t_start >= t_end) continue;  // only positions before its first tile
-    t_start += tile0;
-    t_end += tile0;
-    return true;
+    if (any) return true;
   }
   return false;
 }
@@ -537,7 +552,9 @@ hipError_t launch_partial_fp8(const PartialArgs& a, dim3 grid, int dtype, bool p
 hipError_t launch_partial_g16(const PartialArgs& a, dim3 grid, int dtype, bool paged, hipStream_t stream);
 
 // Stage 1 over shared prefixes (mla_decode.hip): grid = workers; uni: pages
-// of a power of two of whole 32-token sub-tiles (an fp8 cache needs them).
-hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, bool fp8, hipStream_t stream);
+// of a power of two of whole 32-token sub-tiles (an fp8 cache needs them);
+// fused: the workers make the plan themselves.
+hipError_t launch_partial_shared(const SharedFusedArgs& a, int dtype, bool uni, bool fp8, bool fused,
+                                 hipStream_t stream);
 
 }  // namespace tmla

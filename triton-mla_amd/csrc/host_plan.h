@@ -374,16 +374,22 @@ inline int64_t shared_prefix_items(int64_t batch, int64_t rows, int64_t groups) 
 }
 inline int64_t shared_own_items(int64_t batch, int64_t rows) { return batch * ((rows + 127) / 128); }
 
+// Whether the workers make the plan themselves, in LDS.
+inline bool shared_small(int64_t batch, int64_t rows, int64_t groups) {
+  return batch <= kSharedSmallBatch && groups <= kSharedSmallBatch &&
+         shared_prefix_items(batch, rows, groups) + shared_own_items(batch, rows) <= kSharedSmallItems;
+}
+
 // Workspace: the plan kernel's output, then the partials' lse values and the
 // partials (512 values of 16 bits a row). Every piece of an item has the
 // item's rows; there are at most workers + items pieces, those of a
 // sequence's own tokens of at most min(rows, 128) rows.
 struct SharedWs {
-  size_t items, merges, worker_first, mid_lse, mid_o;
+  size_t items, merges, worker_first, worker_list, mid_lse, mid_o;
   size_t total;  // 0: invalid or too large
 };
 inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t workers) {
-  SharedWs w{0, 0, 0, 0, 0, 0};
+  SharedWs w{0, 0, 0, 0, 0, 0, 0};
   if (batch < 0 || rows <= 0 || groups <= 0 || workers <= 0) return w;
   if ((int64_t)batch * rows > INT32_MAX / 2) return w;
   const int64_t np = shared_prefix_items(batch, rows, groups), ns = shared_own_items(batch, rows);
@@ -392,7 +398,9 @@ inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t w
   auto al = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   w.items = 256;
   w.worker_first = w.items + (size_t)al((np + ns) * kSharedItemBytes);
-  w.merges = w.worker_first + (size_t)al((int64_t)workers * kSharedItemBytes);
+  w.worker_list = w.worker_first + (size_t)al((int64_t)workers * kSharedItemBytes);
+  w.merges = w.worker_list +
+             (shared_small(batch, rows, groups) ? (size_t)al((int64_t)workers * kSharedSmallItems * kSharedItemBytes) : 0);
   w.mid_lse = w.merges + (size_t)al(ns * kSharedMergeBytes);
   w.mid_o = w.mid_lse + (size_t)al(mid * 4);
   w.total = w.mid_o + (size_t)(mid * 1024);

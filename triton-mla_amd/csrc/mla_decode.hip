@@ -40,6 +40,7 @@
 #include "cdna.h"
 #include "decode_common.h"
 #include "merge.h"
+#include "shared_plan.h"
 #include "triton_mla.h"
 
 namespace tmla {
@@ -430,7 +431,8 @@ struct Segment {
 template <int DT, int DV, int DR, int NHB, bool PAGED, bool PAGE_UNIFORM, bool F8 = false, class Args = PartialArgs>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
 void mla_partial_kernel(Args a) {
-  constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
+  constexpr bool SHARED = std::is_base_of_v<SharedArgs, Args>;
+  constexpr bool FUSED = std::is_same_v<Args, SharedFusedArgs>;  // (SHARED) the workers make the plan
   static_assert(!SHARED || (F8 && NHB == 4), "shared prefixes: 128 rows a workgroup (16-bit caches: mla_partial_own_kernel)");
   constexpr int DQK = DV + DR;
   static_assert(DQK % 64 == 0 && DV % 64 == 0, "row must be whole 128-byte blocks");
@@ -539,9 +541,11 @@ void mla_partial_kernel(Args a) {
 
   // ---- work range -------------------------------------------------------
   WorkRange wr{};
-  SharedWalk walk{};
+  std::conditional_t<FUSED, SharedOwnWalk, SharedWalk> walk{};
+  __shared__ SharedItem s_list[FUSED ? kSharedList : 1];
+  static_assert(!FUSED || sizeof(SharedSmallPlan::Lds) <= SMEM, "the plan fits the rings");
   if constexpr (SHARED) {
-    if (!shared_begin(a, worker, walk)) return;
+    if (!shared_begin(a, worker, walk, smem, s_list)) return;
   } else if (!work_range(a, worker, wr)) {
     if (!fused) return;  // (the fused tail still clears empty sequences)
   }
@@ -572,7 +576,7 @@ void mla_partial_kernel(Args a) {
   while (SHARED || remaining > 0) {
     int n_b, nt_b = 0, t_end;
     if constexpr (SHARED) {
-      if (!shared_next(a, walk, item, b, n_b, t_start, t_end)) break;
+      if (!shared_next(a, worker, walk, item, b, n_b, t_start, t_end, s_list)) break;
       lag_wave = __builtin_amdgcn_readfirstlane(shared_lag(a, item, head_base));
     } else {
       n_b = b == b_first ? n_first : a.seqlens[b];
@@ -1548,7 +1552,8 @@ constexpr int own_step_reads(int t) {
 template <int DT, bool PAGED, bool PAGE_UNIFORM, class Args = PartialArgs>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
 void mla_partial_own_kernel(Args a) {
-  constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
+  constexpr bool SHARED = std::is_base_of_v<SharedArgs, Args>;
+  constexpr bool FUSED = std::is_same_v<Args, SharedFusedArgs>;  // (SHARED) the workers make the plan
   constexpr int DV = 512, DQK = 576;
   constexpr int NCB = DQK / 64;   // 128-byte column blocks per row
   constexpr int NVB = DV / 64;    // ... of which hold V dims
@@ -1631,9 +1636,11 @@ void mla_partial_own_kernel(Args a) {
 
   // ---- work range -------------------------------------------------------
   WorkRange wr{};
-  SharedWalk walk{};
+  std::conditional_t<FUSED, SharedOwnWalk, SharedWalk> walk{};
+  __shared__ SharedItem s_list[FUSED ? kSharedList : 1];
+  static_assert(!FUSED || sizeof(SharedSmallPlan::Lds) <= SMEM, "the plan fits the rings");
   if constexpr (SHARED) {
-    if (!shared_begin(a, worker, walk)) return;
+    if (!shared_begin(a, worker, walk, smem, s_list)) return;
   } else if (!work_range(a, worker, wr)) {
     if (!fused) return;
   }
@@ -1662,7 +1669,7 @@ void mla_partial_own_kernel(Args a) {
   while (SHARED || remaining > 0) {
     int n_b, nt_b = 0, t_end;
     if constexpr (SHARED) {
-      if (!shared_next(a, walk, item, b, n_b, t_start, t_end)) break;
+      if (!shared_next(a, worker, walk, item, b, n_b, t_start, t_end, s_list)) break;
       lag_wave = __builtin_amdgcn_readfirstlane(shared_lag(a, item, head_base));
     } else {
       n_b = b == b_first ? n_first : a.seqlens[b];
@@ -2312,21 +2319,26 @@ hipError_t launch_partial_own_t(const PartialArgs& a, dim3 grid, hipStream_t str
   return hipGetLastError();
 }
 
-template <int DT>
-hipError_t launch_partial_shared_t(const SharedArgs& a, int workers, bool uni, bool fp8, hipStream_t stream) {
+template <int DT, class Args>
+hipError_t launch_partial_shared_t(const Args& a, bool uni, bool fp8, hipStream_t stream) {
+  const dim3 grid(a.num_workers), block(256);
   if (fp8)
-    hipLaunchKernelGGL((mla_partial_kernel<DT, 512, 64, 4, true, true, true, SharedArgs>), dim3(workers), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL((mla_partial_kernel<DT, 512, 64, 4, true, true, true, Args>), grid, block, 0, stream, a);
   else if (uni)
-    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, true, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, true, Args>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, false, SharedArgs>), dim3(workers), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((mla_partial_own_kernel<DT, true, false, Args>), grid, block, 0, stream, a);
   return hipGetLastError();
 }
 
-hipError_t launch_partial_shared(const SharedArgs& a, int workers, int dtype, bool uni, bool fp8, hipStream_t stream) {
-  return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(a, workers, uni, fp8, stream)
-                            : launch_partial_shared_t<TMLA_FP16>(a, workers, uni, fp8, stream);
+hipError_t launch_partial_shared(const SharedFusedArgs& a, int dtype, bool uni, bool fp8, bool fused,
+                                 hipStream_t stream) {
+  const SharedArgs& p = a;
+  if (fused)
+    return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(a, uni, fp8, stream)
+                              : launch_partial_shared_t<TMLA_FP16>(a, uni, fp8, stream);
+  return dtype == TMLA_BF16 ? launch_partial_shared_t<TMLA_BF16>(p, uni, fp8, stream)
+                            : launch_partial_shared_t<TMLA_FP16>(p, uni, fp8, stream);
 }
 
 template <int DT>

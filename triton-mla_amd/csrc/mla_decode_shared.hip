@@ -25,6 +25,7 @@
 #include "decode_common.h"
 #include "host_plan.h"
 #include "merge.h"
+#include "shared_plan.h"
 
 namespace tmla {
 
@@ -32,280 +33,20 @@ int hip_fail(hipError_t e, const char* where);
 
 namespace {
 
-struct PlanArgs {
-  const int32_t* seqlens;
-  const int32_t* prefix_lens;   // [groups], or null: prefix_len for each
-  const int32_t* group_starts;  // [groups + 1], or null: one group of the whole batch
-  int32_t prefix_len, groups, batch, rows_per_seq, q_len, capacity, workers;
-  SharedHeader* header;
-  SharedItem* items;
-  SharedItem* worker_first;  // [workers]
-  SharedMerge* merges;       // [batch, blocks of 128 rows]
-};
-
-// Inclusive maximum over the lanes of a wave (as wave_scan: by DPP moves); x >= 0.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_imax(int x) {
-  return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false));
-}
-__device__ __forceinline__ int wave_scan_max(int x) {
-  x = dpp_imax<0x111, 0xF>(x);
-  x = dpp_imax<0x112, 0xF>(x);
-  x = dpp_imax<0x114, 0xF>(x);
-  x = dpp_imax<0x118, 0xF>(x);
-  x = dpp_imax<0x142, 0xA>(x);
-  return dpp_imax<0x143, 0xC>(x);
-}
-
-// Scans over the T threads of a workgroup in turns of one barrier each: a scan
-// writes the sums that its predecessor did not, which every thread has read
-// by the time of the scan after next.
-template <int T>
-struct Scanner {
-  int (*sums)[T / 64];
-  int turn = 0;
-  // values in front of this thread (of x >= 0: sum or maximum); total of all
-  template <bool MAX>
-  __device__ __forceinline__ int before(int x, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int incl = MAX ? wave_scan_max(x) : wave_scan(x);
-    int* s = sums[turn];
-    turn ^= 1;
-    if (lane == 63) s[wave] = incl;
-    __syncthreads();
-    int head = 0;
-    total = 0;
-    for (int w = 0; w < T / 64; ++w) {
-      const int v = s[w];
-      if (w < wave) head = MAX ? max(head, v) : head + v;
-      total = MAX ? max(total, v) : total + v;
-    }
-    return MAX ? max(head, incl) : head + incl - x;  // (MAX: with this thread)
+// The plan of calls too large for the workers to make it themselves.
+__global__ __launch_bounds__(1024) void mla_shared_plan_kernel(SharedArgs p) {
+  constexpr int T = 1024;
+  using Plan = SharedPlan<T, false>;
+  __shared__ Plan::Lds lds;
+  Plan plan(p, lds);
+  plan.make();
+  const int tid = threadIdx.x;
+  if (tid == 0) *p.header = SharedHeader{plan.n_items, plan.chunk, plan.line};
+  for (int w = tid; w < p.num_workers && w * plan.chunk < plan.line; w += T) {
+    const int i = plan.first_item(w);
+    plan.write(p.worker_first + w, i, plan.place(i), plan.pos_of(i), plan.mid_of(i));
   }
-};
-
-// Last index i of the ascending a[0..n] with a[i] <= x (a[0] <= x).
-template <class F>
-__device__ __forceinline__ int last_at_most(F&& a, int n, int x) {
-  int lo = 0, hi = n + 1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a(mid) <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// One workgroup makes the plan: what it costs is its chain of loads and
-// barriers, so the lengths and bounds are loaded at once and everything else
-// stays in LDS (SMALL), four waves. 64 sequences of one group: PLAN_US us. Calls
-// beyond kSharedSmall... keep lengths and items in memory, with 16 waves.
-template <bool SMALL>
-__global__ __launch_bounds__(SMALL ? 256 : 1024) void mla_shared_plan_kernel(PlanArgs p) {
-  constexpr int T = SMALL ? 256 : 1024;
-  constexpr int GROUPS = SMALL ? kSharedSmallBatch : kSharedMaxGroups;
-  __shared__ int s_start[GROUPS + 1];  // first sequence of each group, ascending
-  __shared__ int s_tiles[GROUPS];      // prefix tokens, then prefix tiles of each group
-  __shared__ int s_first[GROUPS];      // the group's first sequence that holds a token
-  __shared__ int s_base[GROUPS + 1];   // its first prefix item
-  __shared__ int s_sums[2][T / 64];
-  __shared__ int s_len[SMALL ? kSharedSmallBatch : 1];
-  __shared__ int s_pos[SMALL ? kSharedSmallItems : 1], s_mid[SMALL ? kSharedSmallItems : 1];
-  const int tid = threadIdx.x, G = p.groups, R = p.rows_per_seq;
-  Scanner<T> scan{s_sums};
-  int total;
-  // Groups: bounds that are out of order or out of the batch leave groups
-  // shorter or empty, never overlapping.
-  auto bound = [&](int g) {
-    return min(max(p.group_starts ? p.group_starts[g] : (g == 0 ? 0 : p.batch), 0), p.batch);
-  };
-  auto prefix = [&](int g) { return max(p.prefix_lens ? p.prefix_lens[g] : p.prefix_len, 0); };
-  auto load_length = [&](int b) { return min(p.seqlens[b], p.capacity); };
-  auto length = [&](int b) {
-    if constexpr (SMALL) return s_len[b];
-    else return load_length(b);
-  };
-  const int first_prefix = tid < G ? prefix(tid) : 0;
-  if constexpr (SMALL) {
-    if (tid < p.batch) s_len[tid] = load_length(tid);
-    s_first[tid] = INT32_MAX;
-  }
-  int carry = 0;
-  for (int g0 = 0; g0 <= G; g0 += T) {
-    const int g = g0 + tid;
-    const int v = max(scan.template before<true>(g <= G ? bound(g) : 0, total), carry);
-    if (g <= G) s_start[g] = v;
-    carry = max(carry, total);
-  }
-  for (int g = tid; g < G; g += T) {
-    s_tiles[g] = g == tid ? first_prefix : prefix(g);
-    if constexpr (!SMALL) s_first[g] = INT32_MAX;
-  }
-  __syncthreads();
-  // No row of a group may see fewer tokens than its prefix (but for sequences
-  // that hold nothing, whose rows no prefix partial counts for).
-  auto group_of = [&](int b) {
-    const int g = last_at_most([&](int i) { return s_start[i]; }, G, b);
-    return g < G && b >= s_start[0] ? g : -1;
-  };
-  for (int b = tid; b < p.batch; b += T) {
-    const int n = length(b), g = group_of(b);
-    if (g >= 0 && n > 0) {
-      atomicMin(&s_tiles[g], max(n - (p.q_len - 1), 0));
-      atomicMin(&s_first[g], b);
-    }
-  }
-  __syncthreads();
-  int n_prefix = 0;
-  for (int g0 = 0; g0 < G; g0 += T) {
-    const int g = g0 + tid;
-    int blocks = 0;
-    if (g < G) {
-      // whole tiles (what is left of the prefix each sequence reads itself),
-      // of groups that have somebody to share with
-      const int n = s_start[g + 1] - s_start[g];
-      const int tiles = n < 2 || s_first[g] == INT32_MAX ? 0 : s_tiles[g] / kTileTokens;
-      s_tiles[g] = tiles;
-      if (tiles > 0) blocks = (n * R + kSharedRows - 1) / kSharedRows;
-    }
-    const int at = scan.template before<false>(blocks, total) + n_prefix;
-    if (g < G) s_base[g] = at;
-    n_prefix += total;
-  }
-  if (tid == 0) s_base[G] = n_prefix;
-  __syncthreads();
-  // items and their positions on the line
-  const int per_seq = (R + kSharedRows - 1) / kSharedRows;
-  const int n_items = n_prefix + p.batch * per_seq;
-  struct Place {
-    int row0, rows, seq, tile0, tiles, len;
-  };
-  auto place = [&](int i) {
-    Place x;
-    if (i < n_prefix) {
-      const int g = last_at_most([&](int j) { return s_base[j]; }, G - 1, i);
-      const int lo = (i - s_base[g]) * kSharedRows;
-      x.row0 = s_start[g] * R + lo;
-      x.rows = min(kSharedRows, (s_start[g + 1] - s_start[g]) * R - lo);
-      x.seq = s_first[g];
-      x.tile0 = 0;
-      x.tiles = s_tiles[g];
-      x.len = x.tiles * kTileTokens;
-    } else {
-      x.seq = (i - n_prefix) / per_seq;
-      const int lo = (i - n_prefix - x.seq * per_seq) * kSharedRows;
-      const int g = group_of(x.seq);
-      x.row0 = x.seq * R + lo;
-      x.rows = min(kSharedRows, R - lo);
-      x.len = length(x.seq);
-      x.tile0 = g >= 0 ? s_tiles[g] : 0;
-      x.tiles = max(tiles_of(x.len) - x.tile0, 0);
-    }
-    return x;
-  };
-  int line = 0;
-  for (int i0 = 0; i0 < n_items; i0 += T) {
-    const int i = i0 + tid;
-    int span = 0;
-    if (i < n_items) {
-      const int tiles = place(i).tiles;
-      span = tiles > 0 ? tiles + kSegCostTiles : 0;
-    }
-    const int pos = scan.template before<false>(span, total) + line + kSegCostTiles;
-    if (i < n_items) {
-      if constexpr (SMALL) s_pos[i] = pos;
-      else p.items[i].pos = pos;
-    }
-    line += total;
-  }
-  const int chunk = max((line + p.workers - 1) / p.workers, 1);
-  if (tid == 0) *p.header = SharedHeader{n_items, chunk, line};
-  auto pos_of = [&](int i) {
-    if constexpr (SMALL) return s_pos[i];
-    else return p.items[i].pos;
-  };
-  auto pieces_of = [&](int pos, int tiles) { return tiles > 0 ? (pos + tiles - 1) / chunk - pos / chunk + 1 : 0; };
-  int rows_line = 0;
-  for (int i0 = 0; i0 < n_items; i0 += T) {
-    const int i = i0 + tid;
-    Place x{};
-    int pos = 0, pieces = 0;
-    if (i < n_items) {  // (pos: this thread's own)
-      x = place(i);
-      pos = pos_of(i);
-      pieces = pieces_of(pos, x.tiles);
-    }
-    const int mid = scan.template before<false>(pieces * x.rows, total) + rows_line;
-    if (i < n_items) {
-      SharedItem* it = p.items + i;
-      it->row0 = x.row0;
-      it->rows = x.rows;
-      it->seq = x.seq;
-      it->tile0 = x.tile0;
-      it->tiles = x.tiles;
-      it->len = x.len;
-      it->causal = i >= n_prefix;
-      it->pos = pos;
-      it->first_worker = pos / chunk;
-      it->pieces = pieces;
-      it->mid_row = mid;
-      it->index = i;
-      if constexpr (SMALL) s_mid[i] = mid;
-    }
-    rows_line += total;
-  }
-  if constexpr (!SMALL) __threadfence();  // the items, for the other waves
-  __syncthreads();
-  auto mid_of = [&](int i) {
-    if constexpr (SMALL) return s_mid[i];
-    else return p.items[i].mid_row;
-  };
-  // the item that each worker's range begins in: the last whose positions
-  // (with those before its first tile) begin at or before it
-  for (int w = tid; w < p.workers; w += T) {
-    const int lo = w * chunk;
-    if (lo >= line) break;
-    const int i = last_at_most([&](int j) { return pos_of(j) - kSegCostTiles; }, n_items - 1, lo);
-    const Place x = place(i);
-    SharedItem* it = p.worker_first + w;
-    const int pos = pos_of(i);
-    it->row0 = x.row0;
-    it->rows = x.rows;
-    it->seq = x.seq;
-    it->tile0 = x.tile0;
-    it->tiles = x.tiles;
-    it->len = x.len;
-    it->causal = i >= n_prefix;
-    it->pos = pos;
-    it->first_worker = pos / chunk;
-    it->mid_row = mid_of(i);
-    it->index = i;
-  }
-  // where each block of rows finds its partials
-  for (int i = n_prefix + tid; i < n_items; i += T) {
-    const Place x = place(i);
-    const int g = group_of(x.seq);
-    SharedMerge m{};
-    m.own_row = mid_of(i);
-    m.own_rows = x.rows;
-    m.own_pieces = pieces_of(pos_of(i), x.tiles);
-    m.split = kSharedRows;
-    if (g >= 0 && s_tiles[g] > 0 && x.len > 0) {
-      const int row = x.row0 - s_start[g] * R, at = row % kSharedRows;
-      for (int k = 0; k < 2; ++k) {
-        const int j = s_base[g] + row / kSharedRows + k;
-        if (k == 1) {
-          m.split = kSharedRows - at;
-          if (m.split >= x.rows) break;
-        }
-        const Place y = place(j);
-        m.rows[k] = y.rows;
-        m.pieces[k] = pieces_of(pos_of(j), y.tiles);
-        m.row[k] = mid_of(j) + (k == 0 ? at : -m.split);
-      }
-    }
-    p.merges[i - n_prefix] = m;
-  }
+  for (int i = plan.n_prefix + tid; i < plan.n_items; i += T) plan.write_merge(i);
 }
 
 struct SharedCombineArgs {
@@ -407,32 +148,8 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
   const int32_t rows = q_len * num_heads;
   const SharedWs w = shared_ws(batch, rows, num_groups, num_workers);
   char* ws = static_cast<char*>(workspace);
-  PlanArgs p{};
-  p.seqlens = cache_seqlens;
-  p.prefix_lens = prefix_lens;
-  p.group_starts = group_starts;
-  p.prefix_len = prefix_len;
-  p.groups = num_groups;
-  p.batch = batch;
-  p.rows_per_seq = rows;
-  p.q_len = q_len;
-  p.capacity = shared_capacity(c);
-  p.workers = num_workers;
-  p.header = reinterpret_cast<SharedHeader*>(ws);
-  p.items = reinterpret_cast<SharedItem*>(ws + w.items);
-  p.worker_first = reinterpret_cast<SharedItem*>(ws + w.worker_first);
-  p.merges = reinterpret_cast<SharedMerge*>(ws + w.merges);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool small = batch <= kSharedSmallBatch && num_groups <= kSharedSmallBatch &&
-                     shared_prefix_items(batch, rows, num_groups) + shared_own_items(batch, rows) <= kSharedSmallItems;
-  if (small)
-    hipLaunchKernelGGL(mla_shared_plan_kernel<true>, dim3(1), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL(mla_shared_plan_kernel<false>, dim3(1), dim3(1024), 0, s, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return hip_fail(e, "mla_shared_plan_kernel launch");
-
-  SharedArgs a{};
+  SharedFusedArgs a{};
   a.q = static_cast<const char*>(q);
   a.q_sb = q_stride_b;
   a.q_sh = q_stride_h;
@@ -457,18 +174,32 @@ int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
   a.xcds = 1;
   a.mid_o = reinterpret_cast<short*>(ws + w.mid_o);
   a.mid_lse = reinterpret_cast<float*>(ws + w.mid_lse);
-  a.header = p.header;
-  a.items = p.items;
-  a.worker_first = p.worker_first;
+  a.prefix_lens = prefix_lens;
+  a.group_starts = group_starts;
+  a.prefix_len = prefix_len;
+  a.groups = num_groups;
+  a.capacity = shared_capacity(c);
+  a.merges = reinterpret_cast<SharedMerge*>(ws + w.merges);
+  a.header = reinterpret_cast<SharedHeader*>(ws);
+  a.items = reinterpret_cast<SharedItem*>(ws + w.items);
+  a.worker_first = reinterpret_cast<SharedItem*>(ws + w.worker_first);
+  a.worker_list = reinterpret_cast<SharedItem*>(ws + w.worker_list);
   const bool uni = page_size % 32 == 0 && a.page_shift >= 0;
   if (fp8) {
     a.kv_scale = kv_scale;
     a.sc_s0 = scale_stride_0;
   }
-  e = launch_partial_shared(a, num_workers, dtype, uni, fp8, s);
+  const bool fused = shared_small(batch, rows, num_groups);
+  hipError_t e;
+  if (!fused) {
+    hipLaunchKernelGGL(mla_shared_plan_kernel, dim3(1), dim3(1024), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return hip_fail(e, "mla_shared_plan_kernel launch");
+  }
+  e = launch_partial_shared(a, dtype, uni, fp8, fused, s);
   if (e != hipSuccess) return hip_fail(e, "stage 1 launch");
 
-  const SharedCombineArgs ca{p.merges, a.mid_o, a.mid_lse, rows, static_cast<char*>(out), out_stride_b, out_stride_h,
+  const SharedCombineArgs ca{a.merges, a.mid_o, a.mid_lse, rows, static_cast<char*>(out), out_stride_b, out_stride_h,
                              lse};
   const dim3 grid(batch, (rows + 3) / 4);
   if (dtype == TMLA_BF16)
