@@ -508,7 +508,7 @@ def test_serving_run(gpu, fp8):
     def decode(prefix):
         q = torch.randn(batch, heads, 576, generator=g, device="cuda", dtype=torch.bfloat16)
         shared, lse = triton_mla.mla_decode_shared(q, kv, lens, table, prefix, softmax_scale=192 ** -0.5,
-                                                   return_lse=True, kv_scale=scale)
+                                                   return_lse=True, kv_scale=scale, share=True)
         dense = torch.zeros(batch, max(k.shape[0] for k in kept), 576, dtype=torch.bfloat16, device="cuda")
         for b, k in enumerate(kept):
             dense[b, :k.shape[0]] = k
@@ -540,5 +540,5 @@ def test_serving_run(gpu, fp8):
     assert (refs[live.item():] == 0).all() and (refs[:live.item()] > 0).all()
     kv = kv[:live.item()].clone()  # the rest of the pool can go
     again = triton_mla.mla_decode_shared(q, kv, lens, table, 320, softmax_scale=192 ** -0.5, return_lse=True,
-                                         kv_scale=scale[:live.item()] if fp8 else None)
+                                         kv_scale=scale[:live.item()] if fp8 else None, share=True)
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)

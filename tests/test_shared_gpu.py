@@ -101,7 +101,7 @@ def check(args, out, lse, scale=SCALE, kv=None):
 def run(args, **kw):
     import triton_mla
 
-    return triton_mla.mla_decode_shared(**args, softmax_scale=SCALE, return_lse=True, **kw)
+    return triton_mla.mla_decode_shared(**args, softmax_scale=SCALE, return_lse=True, **{"share": True, **kw})
 
 
 CASES = {
@@ -193,7 +193,7 @@ def test_prefix_as_one_number_and_one_group(gpu):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     import triton_mla
 
-    alone = triton_mla.mla_decode_shared(**args, softmax_scale=SCALE)
+    alone = triton_mla.mla_decode_shared(**args, softmax_scale=SCALE, share=True)
     assert torch.equal(alone, want[0])
 
 
@@ -228,7 +228,7 @@ def test_large_scores_and_negative_scale(gpu):
     check(args, *run(args))
     args = build([3], [320], [1, 64, 100], 16)
     for scale in (-SCALE, 0.0, 1.0):
-        got = triton_mla.mla_decode_shared(**args, softmax_scale=scale, return_lse=True)
+        got = triton_mla.mla_decode_shared(**args, softmax_scale=scale, return_lse=True, share=True)
         check(args, *got, scale=scale)
 
 
@@ -325,5 +325,66 @@ def test_empty_batch(gpu):
     q = torch.empty(0, 16, 576, dtype=torch.bfloat16, device="cuda")
     kv = torch.zeros(2, 64, 576, dtype=torch.bfloat16, device="cuda")
     out, lse = triton_mla.mla_decode_shared(q, kv, torch.empty(0, dtype=torch.int32, device="cuda"),
-                                            torch.empty(0, 3, dtype=torch.int32, device="cuda"), 64, return_lse=True)
+                                            torch.empty(0, 3, dtype=torch.int32, device="cuda"), 64, return_lse=True,
+                                            share=True)
     assert out.shape == (0, 16, 512) and lse.shape == (0, 16)
+
+
+@pytest.mark.parametrize("name", ["one_group", "all_heads", "padded_rows", "two_tokens", "five_tokens_short"])
+def test_without_sharing_it_is_mla_decode(gpu, name):
+    import triton_mla
+
+    sizes, prefixes, own, heads, page, dtype, q_len, empty = CASES[name]
+    args = build(sizes, prefixes, own, heads, page, dtype, q_len, empty=empty)
+    plain = triton_mla.mla_decode(args["q"], args["kv_cache"], args["cache_seqlens"], args["block_table"],
+                                  softmax_scale=SCALE, return_lse=True)
+    for share in (False, None):  # (small calls: both run mla_decode)
+        got = run(args, share=share)
+        assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+
+
+def test_sharing_is_chosen_by_size(gpu):
+    """A call past the rule's sizes shares (the bits of share=True)."""
+    args = build([40], [4096], [1 + i for i in range(40)], 16)
+    want = run(args)
+    got = run(args, share=None)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check(args, *got)
+
+
+def test_items_past_the_list_of_a_worker(gpu):
+    """Many short ends behind one prefix: a worker's items do not fit its list."""
+    import triton_mla
+
+    args = build([200], [6400], [1 + i % 3 for i in range(200)], 4)
+    check(args, *run(args))
+    codes, scale = triton_mla.quantize_kv_fp8(args["kv_cache"], "page")
+    check({**args, "kv_cache": codes}, *run({**args, "kv_cache": codes}, kv_scale=scale),
+          kv=triton_mla.dequantize_kv_fp8(codes, scale).double())
+
+
+@pytest.mark.parametrize("batch", [255, 256, 257])
+def test_plans_by_the_workers_and_by_their_own_launch(gpu, batch):
+    """Both sides of the size up to which the workers make the plan."""
+    sizes = [batch - 2, 2]
+    args = build(sizes, [192, 128], [1 + (7 * i) % 90 for i in range(batch)], 20, empty=(3, batch - 1))
+    check(args, *run(args))
+
+
+def test_one_worker_and_many(gpu):
+    """The C entry with other worker counts than the device's."""
+    from triton_mla import _native
+
+    args = build([6, 3], [640, 200], [1, 70, 2, 130, 64, 65, 9, 8, 7], 24)
+    q, kv, bt = args["q"], args["kv_cache"], args["block_table"]
+    lib = _native.load()
+    for workers in (1, 3, 1000):
+        need = lib.tmla_shared_workspace_bytes(9, 24, 2, workers)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        out, lse = torch.empty(9, 24, 512, dtype=q.dtype, device="cuda"), torch.empty(9, 24, device="cuda")
+        _native.check(lib.tmla_mla_decode_shared(
+            q.data_ptr(), q.stride(0), q.stride(1), kv.data_ptr(), kv.stride(0), kv.stride(1), kv.shape[0], 64, None, 0,
+            bt.data_ptr(), bt.stride(0), bt.shape[1], args["cache_seqlens"].data_ptr(), args["prefix_lens"].data_ptr(),
+            0, args["group_starts"].data_ptr(), 2, 9, 1, 24, 512, 64, 0, SCALE, workers, out.data_ptr(), out.stride(0),
+            out.stride(1), lse.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream), "shared")
+        check(args, out, lse)

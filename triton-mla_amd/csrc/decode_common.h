@@ -27,7 +27,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // table's row `seq`: the prefix of a group of sequences, or what one sequence
 // has of its own behind it. On the line that the workers share (as the
 // balanced partition's straddling ranges do) the item's first tile is at
-// `pos`, after kSegCostTiles extra positions. Its pieces' partial rows lie one
+// `pos`, after kSharedSegTiles extra positions. Its pieces' partial rows lie one
 // after another, `rows` each, from mid_row on.
 struct SharedItem {
   int32_t row0, rows;
@@ -524,7 +524,7 @@ __device__ __forceinline__ bool shared_next(const SharedArgs& a, int, SharedWalk
                                             int& t_start, int& t_end, const SharedItem*) {
   while (w.at < w.items) {
     const SharedItem* it = w.next;
-    if (__builtin_amdgcn_readfirstlane(it->pos) - kSegCostTiles >= w.hi) return false;
+    if (__builtin_amdgcn_readfirstlane(it->pos) - kSharedSegTiles >= w.hi) return false;
     const bool any = shared_take(it, w.lo, w.hi, item, b, n_b, t_start, t_end);
     w.at = item.index + 1;
     w.next = a.items + w.at;

@@ -355,6 +355,11 @@ inline int check_generic(const GenericCall& c, const void* workspace, size_t ws_
 // ---------------------------------------------------------------------------
 // Decode over shared prefixes (mla_decode_shared.hip)
 // ---------------------------------------------------------------------------
+// Positions charged for the start of an item (its rows' Q^T, the first tiles'
+// way, the partials' stores), in tiles. Measured with 1 / 2 / 4 / 8: 64 x 16
+// rows over 32K 104 / 94 / 94 / 93 us, fp8 with 16 x 256 rows over 8K 137 / 119 /
+// 115 / 118, 6 x 192 rows over 27K 104 / 89 / 86 / 85.
+constexpr int kSharedSegTiles = 4;
 constexpr int kSharedMaxGroups = 4096;  // what the plan kernel's LDS holds
 constexpr int kSharedMaxWorkers = 65535;
 constexpr int32_t kSharedItemBytes = 64, kSharedMergeBytes = 48;
@@ -433,7 +438,7 @@ inline int check_shared(const SharedCall& c, const void* workspace, size_t ws_by
   const size_t need = shared_ws(c.batch, (int32_t)rows, c.groups, c.workers).total;
   // the line's positions are 32 bits
   const int64_t items = shared_prefix_items(c.batch, rows, c.groups) + shared_own_items(c.batch, rows);
-  const int64_t tiles = (int64_t)shared_capacity(c) / kTileTokens + 1 + kSegCostTiles;
+  const int64_t tiles = (int64_t)shared_capacity(c) / kTileTokens + 1 + kSharedSegTiles;
   if (need == 0 || items * tiles > INT32_MAX - 2 * kSharedMaxWorkers)
     return fail(TMLA_ERR_UNSUPPORTED, "batch, heads and block-table width are too large together");
   if (workspace == nullptr || ws_bytes < need)

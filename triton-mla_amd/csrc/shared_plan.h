@@ -156,7 +156,7 @@ struct SharedPlan {
   // The item that worker w's range begins in: the last whose positions (with
   // those before its first tile) begin at or before it.
   __device__ __forceinline__ int first_item(int w) const {
-    return last_at_most([&](int j) { return pos_of(j) - kSegCostTiles; }, n_items - 1, w * chunk);
+    return last_at_most([&](int j) { return pos_of(j) - kSharedSegTiles; }, n_items - 1, w * chunk);
   }
   // Where the rows of own item i (i >= n_prefix) find their partials.
   __device__ __forceinline__ void write_merge(int i) const {
@@ -245,9 +245,9 @@ struct SharedPlan {
       int span = 0;
       if (i < n_items) {
         const int tiles = place(i).tiles;
-        span = tiles > 0 ? tiles + kSegCostTiles : 0;
+        span = tiles > 0 ? tiles + kSharedSegTiles : 0;
       }
-      const int pos = scan.template before<false>(span, total) + line + kSegCostTiles;
+      const int pos = scan.template before<false>(span, total) + line + kSharedSegTiles;
       if (i < n_items) {
         if constexpr (SMALL) s.pos[i] = pos;
         else p.items[i].pos = pos;
@@ -301,7 +301,7 @@ __device__ __forceinline__ bool shared_begin(const SharedFusedArgs& a, int worke
   if (w.lo < w.hi) {
     const int first = plan.first_item(worker);
     // (the first item beyond the range, by its positions)
-    const int end = last_at_most([&](int j) { return plan.pos_of(j) - kSegCostTiles; }, plan.n_items - 1, w.hi - 1) + 1;
+    const int end = last_at_most([&](int j) { return plan.pos_of(j) - kSharedSegTiles; }, plan.n_items - 1, w.hi - 1) + 1;
     w.count = __builtin_amdgcn_readfirstlane(end - first);
     SharedItem* more = a.worker_list + (int64_t)worker * kSharedSmallItems;
     for (int k = tid; k < w.count; k += 256)

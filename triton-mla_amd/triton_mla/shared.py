@@ -14,6 +14,30 @@ from . import _native
 from . import kernel as _k
 
 
+def _sharing_pays(rows, batch, capacity, fp8):
+    """Whether attending to the prefixes once for their groups is faster than
+    ``mla_decode``, which reads them per sequence: from what the host knows,
+    the rows of a sequence (query tokens x heads) and the cache that a batch of
+    full block tables would read. Measured (us, shared / mla_decode):
+
+      * Sequences whose rows fill whole blocks of 128 leave no matrix work to
+        save, and the bytes of shared pages come from the caches: 32 x 128 heads
+        over 2K 49 / 42, 8K 95 / 87, 32K 294 / 272; 16 x 2 tokens x 128 heads
+        93 / 86; fp8 over 32K 401 / 347.
+      * Otherwise up to a certain number of bytes the merge of two more
+        partials costs more than it saves. 16-bit caches, about 150 MB: 16
+        heads, 41 MB 26 / 22, 153 MB 38 / 37, 155 MB 33 / 35, 317 MB 39 / 50, 2.4
+        GB 94 / 263; 64 heads, 90 MB 43 / 34, 153 MB 44 / 47, 317 MB 66 / 68. fp8,
+        about 75 MB: 32 heads, 45 MB 42 / 34, 76 MB 43 / 49, 158 MB 57 / 75; but
+        more where 16 rows or fewer run the kernel that streams codes for 16
+        heads: 77 MB 38 / 28, 158 MB 46 / 36 (it reads 4.8 TB/s).
+    """
+    if rows % 128 == 0:
+        return False
+    least = 150e6 if not fp8 else 350e6 if rows <= 16 else 75e6
+    return batch * capacity * 576 * (1 if fp8 else 2) >= least
+
+
 def mla_decode_shared(
     q: torch.Tensor,
     kv_cache: torch.Tensor,
@@ -25,6 +49,7 @@ def mla_decode_shared(
     softmax_scale: float = None,
     return_lse: bool = False,
     kv_scale=None,
+    share: bool = None,
 ):
     """``mla_decode`` of a batch whose sequences share prefixes.
 
@@ -53,6 +78,9 @@ def mla_decode_shared(
         kv_scale: scales of an fp8 cache, as ``mla_decode`` takes them, one per
             page or one for the whole cache (scales per token are refused), on
             pages of a power of two of at least 32 tokens.
+        share: True attends to every prefix once, False runs ``mla_decode``,
+            None (default) chooses the faster of the two by the sizes
+            (_sharing_pays).
 
     Returns:
         out [batch, num_heads, head_dim_v] in q.dtype (and lse [batch,
@@ -102,6 +130,8 @@ def mla_decode_shared(
     if softmax_scale is None:
         softmax_scale = d_qk ** -0.5
     device = q.device
+    if share is None:
+        share = _sharing_pays(rows, batch, block_table.shape[-1] * kv_cache.shape[1], fp8)
     cache_seqlens = cache_seqlens.to(device=device, dtype=torch.int32).contiguous()
     assert cache_seqlens.shape == (batch,), "cache_seqlens must be [batch]"
     block_table = block_table.to(device=device, dtype=torch.int32)
@@ -122,6 +152,9 @@ def mla_decode_shared(
         prefix_len = int(prefix_lens)
         if not 0 <= prefix_len < 1 << 31:
             raise ValueError("prefix_lens must be in [0, 2^31)")
+    if not share:
+        return _k.mla_decode(q.unflatten(1, (q_len, num_heads)) if multi_token else q, kv_cache, cache_seqlens,
+                             block_table, head_dim_v, softmax_scale, return_lse=return_lse, kv_scale=kv_scale)
     shape = (batch, q_len, num_heads) if multi_token else (batch, num_heads)
     out = torch.empty(*shape, head_dim_v, dtype=q.dtype, device=device)
     lse = torch.empty(*shape, dtype=torch.float32, device=device) if return_lse else None
