@@ -504,6 +504,47 @@ __device__ __forceinline__ bool shared_take(const SharedItem* it, int lo, int hi
   return true;
 }
 
+// Partials of shared prefixes. A row has few of them (its prefix's and its own
+// tokens'), so that rounded to the 16-bit type they would show in the result:
+// they are stored as 16-bit fractions of the row's largest value, 2^-16 of it off
+// at most (bf16 partials made the result's error 1.5 to 1.8 times that of its
+// own rounding at short contexts, these 1.3 to 1.45: what the probabilities'
+// rounding leaves), with the factor beside the log-sum-exp.
+__device__ __forceinline__ float shared_max(float m, float a, float b) {
+  // (a NaN stays; max of magnitudes)
+  asm volatile("v_maximum3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
+  return m;
+}
+// The same of two accumulators, read from where they are (a copy of the block in
+// VGPRs would be spilled).
+__device__ __forceinline__ float shared_max_acc(float m, float a, float b) {
+  float x, y;
+  asm volatile(
+      "v_accvgpr_read_b32 %1, %3\n\tv_accvgpr_read_b32 %2, %4\n\tv_maximum3_f32 %0, %0, |%1|, |%2|"
+      : "+v"(m), "=&v"(x), "=&v"(y)
+      : "a"(a), "a"(b));
+  return m;
+}
+// (a row of zeros, or below the normal numbers, stays zero)
+__device__ __forceinline__ float shared_unit(float largest) {
+  return largest >= 0x1p-126f ? __builtin_amdgcn_rcpf(largest) : 0.0f;
+}
+__device__ __forceinline__ i16x4 shared_pack(float a, float b, float c, float d, float to_unit) {
+  const auto lo = __builtin_amdgcn_cvt_pknorm_i16(a * to_unit, b * to_unit);
+  const auto hi = __builtin_amdgcn_cvt_pknorm_i16(c * to_unit, d * to_unit);
+  return i16x4{lo[0], lo[1], hi[0], hi[1]};
+}
+// The row's log-sum-exp, and in a SharedArgs call the factor of its fractions.
+template <bool SHARED>
+__device__ __forceinline__ void shared_store_lse(float* mid, int64_t row, float lse2, float largest) {
+  if constexpr (SHARED) {
+    store_through_f32(mid + 2 * row, lse2);
+    store_through_f32(mid + 2 * row + 1, largest * (1.0f / 32767.0f));
+  } else {
+    store_through_f32(mid + row, lse2);
+  }
+}
+
 // A worker's way along the items of a SharedArgs call. The first item comes
 // with the worker's own record, one memory round trip after the kernel's start.
 struct SharedWalk {

@@ -386,7 +386,7 @@ inline bool shared_small(int64_t batch, int64_t rows, int64_t groups) {
 }
 
 // Workspace: the plan kernel's output, then the partials' lse values and the
-// partials (512 values of 16 bits a row). Every piece of an item has the
+// partials (512 fractions of 16 bits a row). Every piece of an item has the
 // item's rows; there are at most workers + items pieces, those of a
 // sequence's own tokens of at most min(rows, 128) rows.
 struct SharedWs {
@@ -407,7 +407,7 @@ inline SharedWs shared_ws(int32_t batch, int32_t rows, int32_t groups, int32_t w
   w.merges = w.worker_list +
              (shared_small(batch, rows, groups) ? (size_t)al((int64_t)workers * kSharedSmallItems * kSharedItemBytes) : 0);
   w.mid_lse = w.merges + (size_t)al(ns * kSharedMergeBytes);
-  w.mid_o = w.mid_lse + (size_t)al(mid * 4);
+  w.mid_o = w.mid_lse + (size_t)al(mid * 8);  // (log-sum-exp and factor of a row)
   w.total = w.mid_o + (size_t)(mid * 1024);
   return w;
 }

@@ -1353,10 +1353,39 @@ void mla_partial_kernel(Args a) {
       {
         // 1/l of every head of the workgroup, for the waves' column slices
         ds_write_b32(lds + OFF_A + ((lane & 31) * 4 + wave) * 4, inv);
+        // SHARED: each row's largest value (before 1 / l) over the waves' dims,
+        // through the idle P buffers: [row % 32][head block][wave]
+        static_assert(!SHARED || 32 * NHB * NW * 4 <= 2 * PSLOT, "row maxima fit the P buffers");
+        if constexpr (SHARED) {
+#pragma unroll
+          for (int hb = 0; hb < NHB; ++hb) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j4 = 0; j4 < NDBW; ++j4) {
+              const f32x16& t = acc[j4 * NHB + hb];
+#pragma unroll
+              for (int r = 0; r < 16; r += 2) m = shared_max_acc(m, t[r], t[r + 1]);
+            }
+            float x = m, y = m;
+            swap_rows32(x, y);
+            m = shared_max(m, x, y);
+            ds_write_b32(lds + OFF_P + (((lane & 31) * NHB + hb) * NW + wave) * 4, m);
+          }
+        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         lds_barrier();
         f32x4 inv4 = ds_read_f32x4(lds + OFF_A + (lane & 31) * 16);
         lgkm_tie_f4<0>(inv4);
+        float row_max[NHB], to_unit[NHB];
+        if constexpr (SHARED) {
+#pragma unroll
+          for (int hb = 0; hb < NHB; ++hb) {
+            f32x4 m4 = ds_read_f32x4(lds + OFF_P + ((lane & 31) * NHB + hb) * NW * 4);
+            lgkm_tie_f4<0>(m4);
+            row_max[hb] = shared_max(shared_max(0.0f, m4[0], m4[1]), m4[2], m4[3]);
+            to_unit[hb] = shared_unit(row_max[hb]);
+          }
+        }
         // The normalised rows go through the idle rings (32*NHB padded rows;
         // the 16-byte pad spreads the lanes' 8-byte writes over all banks),
         // so that every global store then writes one whole row of DV elements.
@@ -1367,8 +1396,13 @@ void mla_partial_kernel(Args a) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
               i16x4 v;
+              if constexpr (SHARED) {
+                const f32x16& t = acc[j4 * NHB + hb];
+                v = shared_pack(t[4 * q4], t[4 * q4 + 1], t[4 * q4 + 2], t[4 * q4 + 3], to_unit[hb]);
+              } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = Elt<DT>::from_float(acc[j4 * NHB + hb][4 * q4 + e] * inv4[hb]);
+                for (int e = 0; e < 4; ++e) v[e] = Elt<DT>::from_float(acc[j4 * NHB + hb][4 * q4 + e] * inv4[hb]);
+              }
               const int dim = wave * (DV / NW) + 32 * j4 + 8 * q4 + 4 * hi;
               *reinterpret_cast<i16x4 LDS_AS*>(lds + (hb * 32 + (lane & 31)) * OPITCH + dim * 2) = v;
             }
@@ -1406,7 +1440,8 @@ void mla_partial_kernel(Args a) {
             if (a.lse) a.lse[(int64_t)b * a.num_heads + head] = has ? lse2 * kLn2 : -INFINITY;
           }
           else
-            store_through_f32(a.mid_lse + (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + head, lse2);
+            shared_store_lse<SHARED>(a.mid_lse, (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + head, lse2,
+                                     SHARED ? row_max[NHB == 4 ? wave : 0] * inv : 0.0f);
         }
         // the next segment refills the rings
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -2126,6 +2161,18 @@ void mla_partial_own_kernel(Args a) {
       // (one accumulator block at a time: moved to VGPRs, scaled, rounded
       // and written before the next block is read)
       char LDS_AS* obuf = lds + wave * 32 * OPITCH;
+      float row_max = 0.0f;  // SHARED: of the row's values before 1 / l
+      if constexpr (SHARED) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) row_max = shared_max_acc(row_max, acc[db][r], acc[db][r + 1]);
+        }
+        float x = row_max, y = row_max;
+        swap_rows32(x, y);
+        row_max = shared_max(row_max, x, y);
+      }
+      const float to_unit = shared_unit(row_max);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         f32x16 t = acc[db];
@@ -2133,8 +2180,12 @@ void mla_partial_own_kernel(Args a) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           i16x4 v;
+          if constexpr (SHARED) {
+            v = shared_pack(t[4 * q4], t[4 * q4 + 1], t[4 * q4 + 2], t[4 * q4 + 3], to_unit);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = Elt<DT>::from_float(t[4 * q4 + e] * inv);
+            for (int e = 0; e < 4; ++e) v[e] = Elt<DT>::from_float(t[4 * q4 + e] * inv);
+          }
           const int dim = 32 * db + 8 * q4 + 4 * h2;
           *reinterpret_cast<i16x4 LDS_AS*>(obuf + (ln & 31) * OPITCH + dim * 2) = v;
         }
@@ -2167,7 +2218,8 @@ void mla_partial_own_kernel(Args a) {
           if (a.lse) a.lse[(int64_t)b * a.num_heads + hq] = has ? lse2 * kLn2 : -INFINITY;
         }
         else
-          store_through_f32(a.mid_lse + (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + hq, lse2);
+          shared_store_lse<SHARED>(a.mid_lse, (SHARED ? item.mid_row : 0) + (int64_t)seg.slot * item_rows + hq, lse2,
+                                   row_max * inv);
       }
       // the next segment refills the rings
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -79,27 +79,30 @@ __global__ __launch_bounds__(256) void mla_shared_combine_kernel(SharedCombineAr
     merge_zero(mv, b, head, lane);
     return;
   }
-  const PlainLoads ld{a.mid_o, a.mid_lse};
+  const PlainLoads ld{a.mid_o, nullptr};
+  // (log-sum-exp, factor) of a row's partials
+  auto lse_of = [&](int j) { return reinterpret_cast<const float2*>(a.mid_lse)[row_of(j)]; };
   constexpr int NR = 16;  // rows in flight
   float top = 0.0f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, wsum = 0.0f;
   for (int j0 = 0; j0 < count; j0 += NR) {
     i16x8 v[NR];
-    const float lv = ld.lse(row_of(min(j0 + lane % NR, count - 1)));
+    const float2 lv = lse_of(min(j0 + lane % NR, count - 1));
 #pragma unroll
     for (int j = 0; j < NR; ++j) v[j] = ld.rowv(row_of(min(j0 + j, count - 1)), lane);
     if (j0 == 0) {
-      float x = lv;  // (lanes past the last partial repeat it)
-      for (int j = NR + lane; j < count; j += 64) x = fmaxf(x, ld.lse(row_of(j)));
+      float x = lv.x;  // (lanes past the last partial repeat it)
+      for (int j = NR + lane; j < count; j += 64) x = fmaxf(x, lse_of(j).x);
       top = group_max<64>(x);
       if (top == -INFINITY) top = 0.0f;
     }
-    const float w = j0 + lane % NR < count ? fast_exp2(lv - top) : 0.0f;
+    const float w = j0 + lane % NR < count ? fast_exp2(lv.x - top) : 0.0f;
+    const float ws = w * lv.y;
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      const float wj = lane_value(w, j);
-      wsum += wj;
+      wsum += lane_value(w, j);
+      const float wj = lane_value(ws, j);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += wj * Elt<DT>::to_float(v[j][e]);
+      for (int e = 0; e < 8; ++e) acc[e] += wj * (float)v[j][e];
     }
   }
   merge_store<DT>(mv, b, head, acc, wsum, top, lane);

@@ -31,7 +31,12 @@ def _sharing_pays(rows, batch, capacity, fp8):
         about 75 MB: 32 heads, 45 MB 42 / 34, 76 MB 43 / 49, 158 MB 57 / 75; but
         more where 16 rows or fewer run the kernel that streams codes for 16
         heads: 77 MB 38 / 28, 158 MB 46 / 36 (it reads 4.8 TB/s).
+      * Under 4,096 tokens a row has few partials, and mla_decode's, rounded to
+        the 16-bit type, show in the result (1.5 to 1.9 times the error of its own
+        rounding, 1.3 to 1.45 here): those calls share whatever their size.
     """
+    if capacity < 4096:
+        return True
     if rows % 128 == 0:
         return False
     least = 150e6 if not fp8 else 350e6 if rows <= 16 else 75e6
