@@ -9,11 +9,14 @@
 // lse = log sum_i e^{lse_i}. So the rows of all sequences of a group (row =
 // one query token's head of one sequence) form one tall matrix against the
 // group's prefix, 128 rows to a workgroup, and each sequence's rows meet only
-// its own tokens behind it. Three launches:
-//   1. mla_shared_plan_kernel: lengths and groups -> work items and their
-//      places on the line that the workers share;
-//   2. mla_partial_own_kernel<..., SharedArgs> (mla_decode.hip): the items' partials;
-//   3. mla_shared_combine_kernel: the log-sum-exp merge of each row's partials.
+// its own tokens behind it. Two launches:
+//   1. mla_partial_own_kernel<..., SharedFusedArgs> (mla_decode.hip; fp8 caches
+//      mla_partial_kernel): every worker plans the call (shared_plan.h: lengths
+//      and groups -> work items and their places on the line that the workers
+//      share) and makes the partials of its part of the line;
+//   2. mla_shared_combine_kernel: the log-sum-exp merge of each row's partials.
+// Above 256 sequences or groups or 512 items mla_shared_plan_kernel makes the
+// plan once, in a launch of its own before them (SharedArgs).
 // Reading a prefix once per 128 rows turns the cache's bytes into matrix
 // work: 64 sequences of 16 heads over 32K tokens need 73 GFLOP against 38 MB
 // of prefix instead of 2.4 GB.

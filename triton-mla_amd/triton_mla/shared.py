@@ -14,7 +14,7 @@ from . import _native
 from . import kernel as _k
 
 
-def _sharing_pays(rows, batch, capacity, fp8):
+def _sharing_pays(rows, batch, groups, capacity, fp8):
     """Whether attending to the prefixes once for their groups is faster than
     ``mla_decode``, which reads them per sequence: from what the host knows,
     the rows of a sequence (query tokens x heads) and the cache that a batch of
@@ -31,11 +31,13 @@ def _sharing_pays(rows, batch, capacity, fp8):
         about 75 MB: 32 heads, 45 MB 42 / 34, 76 MB 43 / 49, 158 MB 57 / 75; but
         more where 16 rows or fewer run the kernel that streams codes for 16
         heads: 77 MB 38 / 28, 158 MB 46 / 36 (it reads 4.8 TB/s).
-      * Under 4,096 tokens a row has few partials, and mla_decode's, rounded to
-        the 16-bit type, show in the result (1.5 to 1.9 times the error of its own
-        rounding, 1.3 to 1.45 here): those calls share whatever their size.
+      * Under 4,096 tokens (fp8: 8,192) a row has few partials, and mla_decode's,
+        rounded to the 16-bit type, show in the result (1.5 to 1.9 times the error
+        of its own rounding, 1.0 to 1.4 here): those calls share whatever their
+        size, and so do those of several groups, whose sequences may be short in
+        a long table.
     """
-    if capacity < 4096:
+    if groups > 1 or capacity < (8192 if fp8 else 4096):
         return True
     if rows % 128 == 0:
         return False
@@ -60,8 +62,8 @@ def mla_decode_shared(
 
     The batch is cut into groups of consecutive sequences; the first tokens of
     a group's sequences lie in the same pages, and the group attends to them
-    once. The result is ``mla_decode``'s, up to the rounding of its split
-    partials.
+    once. The result is ``mla_decode``'s, up to the rounding of split
+    partials (finer here, see csrc/mla_decode_shared.hip).
 
     Args:
         q, kv_cache, cache_seqlens, head_dim_v, softmax_scale, return_lse:
@@ -84,8 +86,8 @@ def mla_decode_shared(
             page or one for the whole cache (scales per token are refused), on
             pages of a power of two of at least 32 tokens.
         share: True attends to every prefix once, False runs ``mla_decode``,
-            None (default) chooses the faster of the two by the sizes
-            (_sharing_pays).
+            None (default) chooses by the sizes: mla_decode where it is the
+            faster of the two and its contexts are long (_sharing_pays).
 
     Returns:
         out [batch, num_heads, head_dim_v] in q.dtype (and lse [batch,
@@ -135,8 +137,6 @@ def mla_decode_shared(
     if softmax_scale is None:
         softmax_scale = d_qk ** -0.5
     device = q.device
-    if share is None:
-        share = _sharing_pays(rows, batch, block_table.shape[-1] * kv_cache.shape[1], fp8)
     cache_seqlens = cache_seqlens.to(device=device, dtype=torch.int32).contiguous()
     assert cache_seqlens.shape == (batch,), "cache_seqlens must be [batch]"
     block_table = block_table.to(device=device, dtype=torch.int32)
@@ -157,6 +157,8 @@ def mla_decode_shared(
         prefix_len = int(prefix_lens)
         if not 0 <= prefix_len < 1 << 31:
             raise ValueError("prefix_lens must be in [0, 2^31)")
+    if share is None:
+        share = _sharing_pays(rows, batch, groups, block_table.shape[1] * kv_cache.shape[1], fp8)
     if not share:
         return _k.mla_decode(q.unflatten(1, (q_len, num_heads)) if multi_token else q, kv_cache, cache_seqlens,
                              block_table, head_dim_v, softmax_scale, return_lse=return_lse, kv_scale=kv_scale)
