@@ -572,8 +572,8 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_fill_kernel(Tables t) 
 // Fork, free or reserve by one workgroup, the counts and the rows' values in
 // LDS: tables of at most kPagesSmallEntries entries and pools of at most
 // kPagesSmallPages pages. One launch (and the copies') instead of three or
-// four: a call that reserves for 64 sequences 15.4 us instead of 21.4, a fork
-// into 16 sequences 20.7 instead of 27.
+// four: a call that reserves for 64 sequences 13.9 us instead of 19.9, a fork
+// into 16 sequences 19.1 instead of 25.
 // ---------------------------------------------------------------------------
 enum class Op { kFork, kFree, kReserve };
 constexpr int kSmallThreads = 1024;

@@ -21,6 +21,8 @@ captured into a graph (csrc/cache_pages.hip).
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -35,14 +37,16 @@ def _device_of(*tensors):
 
 
 def _ints(t, name, device, shape=None):
-    t = t.to(device=device, dtype=torch.int32).contiguous()
+    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        t = t.to(device=device, dtype=torch.int32).contiguous()
     if shape is not None:
         assert t.shape == shape, f"{name} must be {list(shape)}"
     return t
 
 
-def _table(block_table, device):
-    block_table = block_table.to(device=device, dtype=torch.int32)
+def _table(block_table):
+    if block_table.dtype is not torch.int32:
+        block_table = block_table.to(torch.int32)
     assert block_table.dim() == 2 and block_table.shape[1] >= 1, "block_table must be [batch, width]"
     return block_table if block_table.stride(1) == 1 else block_table.contiguous()
 
@@ -76,21 +80,27 @@ class _Space:
 
     __slots__ = ("dev_idx", "device", "ws_alloc", "ws_bytes")
 
-    def __init__(self, device, pages, batch, pairs):
-        self.device = device
-        self.dev_idx = device.index if device.index is not None else torch.cuda.current_device()
-        self.ws_bytes = _native.load().tmla_pages_workspace_bytes(pages, batch, pairs)
-        self.ws_alloc = max(self.ws_bytes, 16)
+
+@functools.lru_cache(maxsize=256)
+def _space(device, pages, batch, pairs):
+    space = _Space()
+    space.device = device
+    space.dev_idx = device.index
+    space.ws_bytes = _native.load().tmla_pages_workspace_bytes(pages, batch, pairs)
+    space.ws_alloc = max(space.ws_bytes, 16)
+    return space
 
 
 def _run(name, device, pages, batch, pairs, *args):
     """One C call on the current stream of `device`, with the stream's workspace
     (the GIL is held over its launches, as for the decode calls that share it)."""
-    space = _Space(device, pages, batch, pairs)
+    space = _space(device, pages, batch, pairs)
     with _k._OnDevice(space.dev_idx):
         stream = _k._raw_stream(space.dev_idx)
         ws, ws_ptr = _k._workspace(space, stream)
-        _native.check(getattr(_native.load_gil_held(), name)(*args, ws_ptr, space.ws_bytes, stream), name)
+        rc = getattr(_native.load_gil_held(), name)(*args, ws_ptr, space.ws_bytes, stream)
+    if rc:
+        _native.check(rc, name)
 
 
 def copy_pages(kv_cache, src, dst, kv_scale=None):
@@ -143,7 +153,7 @@ def fork_sequences(kv_cache, block_table, cache_seqlens, page_refs, parents, kv_
         were, nothing is done: the state returned is the one given.
     """
     device = _device_of(kv_cache, block_table, page_refs)
-    table = _table(block_table, device)
+    table = _table(block_table)
     batch, width = table.shape
     pool = _pool(kv_cache, kv_scale)
     seqlens = _ints(cache_seqlens, "cache_seqlens", device, (batch,))
@@ -164,7 +174,7 @@ def free_sequences(block_table, cache_seqlens, page_refs, ended):
 
     Returns (block_table, cache_seqlens, page_refs), the new state."""
     device = _device_of(block_table, page_refs)
-    table = _table(block_table, device)
+    table = _table(block_table)
     batch, width = table.shape
     seqlens = _ints(cache_seqlens, "cache_seqlens", device, (batch,))
     assert page_refs.dim() == 1, "page_refs must be [num_pages]"
@@ -195,7 +205,7 @@ def reserve_pages(block_table, cache_seqlens, page_refs, new_tokens, page_size):
         given.
     """
     device = _device_of(block_table, page_refs)
-    table = _table(block_table, device)
+    table = _table(block_table)
     batch, width = table.shape
     seqlens = _ints(cache_seqlens, "cache_seqlens", device, (batch,))
     assert page_refs.dim() == 1, "page_refs must be [num_pages]"
@@ -226,7 +236,7 @@ def compact_pages(kv_cache, block_table, page_refs, kv_scale=None):
         device: every page from L on is free.
     """
     device = _device_of(kv_cache, block_table, page_refs)
-    table = _table(block_table, device)
+    table = _table(block_table)
     batch, width = table.shape
     pool = _pool(kv_cache, kv_scale)
     refs = _ints(page_refs, "page_refs", device, (pool[3],))

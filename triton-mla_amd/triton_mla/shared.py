@@ -8,6 +8,8 @@ attend to those pages once (csrc/mla_decode_shared.hip).
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -43,6 +45,22 @@ def _sharing_pays(rows, batch, groups, capacity, fp8):
         return False
     least = 150e6 if not fp8 else 350e6 if rows <= 16 else 75e6
     return batch * capacity * 576 * (1 if fp8 else 2) >= least
+
+
+def _ints(t, device):
+    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        t = t.to(device=device, dtype=torch.int32).contiguous()
+    return t
+
+
+@functools.lru_cache(maxsize=256)
+def _space(device, batch, rows, groups, workers):
+    """What kernel._workspace takes to hand out the stream's workspace."""
+    space = _k._CallShape()
+    space.dev_idx, space.device = device.index, device
+    space.ws_bytes = _native.load().tmla_shared_workspace_bytes(batch, rows, groups, workers)
+    space.ws_alloc = max(space.ws_bytes, 16)
+    return space
 
 
 def mla_decode_shared(
@@ -137,20 +155,21 @@ def mla_decode_shared(
     if softmax_scale is None:
         softmax_scale = d_qk ** -0.5
     device = q.device
-    cache_seqlens = cache_seqlens.to(device=device, dtype=torch.int32).contiguous()
+    cache_seqlens = _ints(cache_seqlens, device)
     assert cache_seqlens.shape == (batch,), "cache_seqlens must be [batch]"
-    block_table = block_table.to(device=device, dtype=torch.int32)
+    if block_table.dtype is not torch.int32 or block_table.device != device:
+        block_table = block_table.to(device=device, dtype=torch.int32)
     if block_table.stride(-1) != 1:
         block_table = block_table.contiguous()
     assert block_table.dim() == 2 and block_table.shape[0] == batch
     groups, starts_ptr = 1, None
     if group_starts is not None:
-        group_starts = group_starts.to(device=device, dtype=torch.int32).contiguous()
+        group_starts = _ints(group_starts, device)
         assert group_starts.dim() == 1 and group_starts.shape[0] >= 2, "group_starts must be [groups + 1]"
         groups, starts_ptr = group_starts.shape[0] - 1, group_starts.data_ptr()
     prefix_len, prefix_ptr = 0, None
     if torch.is_tensor(prefix_lens):
-        prefix_lens = prefix_lens.to(device=device, dtype=torch.int32).contiguous()
+        prefix_lens = _ints(prefix_lens, device)
         assert prefix_lens.shape == (groups,), "prefix_lens must be [groups] (or one int)"
         prefix_ptr = prefix_lens.data_ptr()
     else:
@@ -178,19 +197,17 @@ def mla_decode_shared(
             scale_ptr = kv_scale.data_ptr()
         lib = _native.load_gil_held()  # the stream's workspace is shared by its calls
         workers = _k._num_sms(device)
-        call = _k._CallShape()
-        call.dev_idx = device.index if device.index is not None else torch.cuda.current_device()
-        call.device = device
-        call.ws_bytes = lib.tmla_shared_workspace_bytes(batch, rows, groups, workers)
-        call.ws_alloc = max(call.ws_bytes, 16)
+        call = _space(device, batch, rows, groups, workers)
         with _k._OnDevice(call.dev_idx):
             stream = _k._raw_stream(call.dev_idx)
             ws, ws_ptr = _k._workspace(call, stream)
-            _native.check(lib.tmla_mla_decode_shared(
+            rc = lib.tmla_mla_decode_shared(
                 q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1),
                 kv_cache.shape[0], kv_cache.shape[1], scale_ptr, scale_stride, block_table.data_ptr(), block_table.stride(0),
                 block_table.shape[1], cache_seqlens.data_ptr(), prefix_ptr, prefix_len, starts_ptr, groups, batch,
                 q_len, num_heads, head_dim_v, d_rope, _native.DTYPE_CODE[q.dtype], float(softmax_scale), workers,
                 out.data_ptr(), out.stride(0), out.stride(-2), None if lse is None else lse.data_ptr(), ws_ptr,
-                call.ws_bytes, stream), "tmla_mla_decode_shared")
+                call.ws_bytes, stream)
+        if rc:
+            _native.check(rc, "tmla_mla_decode_shared")
     return (out, lse) if return_lse else out
