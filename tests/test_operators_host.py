@@ -80,6 +80,7 @@ def _shared(lib, **kw):
     ({"kv_scale": FAKE, "s1": 584}, 1, b"multiples of 16"), ({"kv_scale": FAKE + 2}, 1, b"aligned"),
     ({"kv_scale": FAKE, "page": 16}, 2, b"32 tokens"), ({"kv_scale": FAKE, "page": 96}, 2, b"32 tokens"),
     ({"heads": 262141}, 2, b"262140"), ({"batch": 1 << 28}, 2, b"too large"),
+    ({"batch": 1 << 24, "heads": 1, "bt_cols": 1}, 2, b"too large"),
     ({"bt_cols": 1 << 30, "batch": 4096}, 2, b"too large"),
 ])
 def test_shared_entry_refusals(lib, kw, status, text):
@@ -146,6 +147,18 @@ def test_page_entries_refuse_bad_tables(lib):
         assert set(got.values()) == {status}, (table, lib.tmla_last_error())
     assert lib.tmla_pages_reserve(FAKE, 3, 2, 3, FAKE, FAKE, 4, 0, None, 1, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == 1
     assert lib.tmla_pages_free(FAKE, 3, 2, 3, FAKE, FAKE, 0, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == 1
+
+
+def test_copies_beyond_a_launch_are_refused(lib):
+    """2^32 threads or more along the grid (pages of 2^30 + 2^20 bytes in rows of an odd
+    number are 1,049,600 workgroups each)."""
+    pool = _pool_args(page=1 << 20, dim=1025, elem=1, s1=1025, s0=1025 << 20, pages=2048)
+    tail = (FAKE, 1 << 40, None)
+    assert lib.tmla_pages_copy(*pool, FAKE, FAKE, 253, FAKE, *tail) == 2
+    assert b"pages of too many bytes" in lib.tmla_last_error()
+    table = (FAKE, 3, 1 << 12, 3)
+    assert lib.tmla_pages_fork(*pool, *table, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, *tail) == 2
+    assert b"pages of too many bytes" in lib.tmla_last_error()
 
 
 def test_pages_workspace(lib):

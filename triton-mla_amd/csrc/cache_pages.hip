@@ -39,6 +39,7 @@ constexpr int kCopyUnits = 4;       // units per thread and part of a page
 constexpr int kFusedPairs = 256;    // copy: pairs that one launch checks and copies
 constexpr int kMarkThreads = 1024;
 constexpr int kCopyGrid = 8192;     // workgroups of a copy, at most
+constexpr int kMaxGrid = (1 << 24) - 1;  // workgroups of a launch of kThreads: fewer than 2^32 threads
 
 // Pages in units of `unit` bytes (16, 4, 2 or 1: what strides and alignment
 // allow); strides in bytes.
@@ -899,7 +900,7 @@ int tmla_pages_copy(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t 
   if (!refused || (pairs > 0 && (!src || !dst))) return fail(TMLA_ERR_INVALID_ARGUMENT, "null pointer argument");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (pairs <= kFusedPairs) {
-    if ((int64_t)pairs * p.parts >= INT32_MAX) return fail(TMLA_ERR_UNSUPPORTED, "pages of too many bytes");
+    if ((int64_t)pairs * p.parts + 1 > kMaxGrid) return fail(TMLA_ERR_UNSUPPORTED, "pages of too many bytes");
     hipLaunchKernelGGL(pages_copy_few_kernel, dim3(pairs * p.parts + 1), dim3(kThreads), 0, s, p, src, dst, pairs,
                        refused);
     TMLA_LAUNCHED("pages_copy_few_kernel");
@@ -933,7 +934,7 @@ int tmla_pages_fork(void* kv, int64_t kv_stride_0, int64_t kv_stride_1, int64_t 
   if (rc != TMLA_OK) return rc;
   if (!refs || !new_refs || !missing || (batch > 0 && (!table || !seqlens || !parents || !new_table || !new_seqlens)))
     return fail(TMLA_ERR_INVALID_ARGUMENT, "null pointer argument");
-  if ((int64_t)batch * p.parts > INT32_MAX) return fail(TMLA_ERR_UNSUPPORTED, "pages of too many bytes for the batch");
+  if ((int64_t)batch * p.parts > kMaxGrid) return fail(TMLA_ERR_UNSUPPORTED, "pages of too many bytes for the batch");
   const PagesWs w = pages_ws(num_pages, batch, 0);
   char* ws = static_cast<char*>(workspace);
   Tables t{};

@@ -439,7 +439,8 @@ inline int check_shared(const SharedCall& c, const void* workspace, size_t ws_by
   // the line's positions are 32 bits
   const int64_t items = shared_prefix_items(c.batch, rows, c.groups) + shared_own_items(c.batch, rows);
   const int64_t tiles = (int64_t)shared_capacity(c) / kTileTokens + 1 + kSharedSegTiles;
-  if (need == 0 || items * tiles > INT32_MAX - 2 * kSharedMaxWorkers)
+  // (a launch has fewer than 2^32 threads along an axis)
+  if (need == 0 || c.batch >= 1 << 24 || items * tiles > INT32_MAX - 2 * kSharedMaxWorkers)
     return fail(TMLA_ERR_UNSUPPORTED, "batch, heads and block-table width are too large together");
   if (workspace == nullptr || ws_bytes < need)
     return fail(TMLA_ERR_WORKSPACE_TOO_SMALL, "workspace is missing or smaller than tmla_shared_workspace_bytes()");
