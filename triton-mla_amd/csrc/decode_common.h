@@ -508,7 +508,7 @@ __device__ __forceinline__ bool shared_take(const SharedItem* it, int lo, int hi
 // tokens'), so that rounded to the 16-bit type they would show in the result:
 // they are stored as 16-bit fractions of the row's largest value, 2^-16 of it off
 // at most (bf16 partials made the result's error 1.5 to 1.8 times that of its
-// own rounding at short contexts, these 1.0 to 1.4: what the probabilities'
+// own rounding at short contexts, these 1.0 to 1.3: what the probabilities'
 // rounding leaves), with the factor beside the log-sum-exp.
 __device__ __forceinline__ float shared_max(float m, float a, float b) {
   // (a NaN stays; max of magnitudes)

@@ -35,7 +35,7 @@ def _sharing_pays(rows, batch, groups, capacity, fp8):
         heads: 77 MB 38 / 28, 158 MB 46 / 36 (it reads 4.8 TB/s).
       * Under 4,096 tokens (fp8: 8,192) a row has few partials, and mla_decode's,
         rounded to the 16-bit type, show in the result (1.5 to 1.9 times the error
-        of its own rounding, 1.0 to 1.4 here): those calls share whatever their
+        of its own rounding, 1.0 to 1.3 here): those calls share whatever their
         size, and so do those of several groups, whose sequences may be short in
         a long table.
     """
