@@ -322,6 +322,32 @@ def test_reserve_more_than_31_bits_are_missing(gpu):
     assert got[2].item() == 2 ** 31 - 1 and got[0].tolist() == rows
 
 
+@pytest.mark.parametrize("pages,every", [(20000, 1), (20001, 2), (14000, 3), (40000, 17), (5_000_000, 1000)])
+def test_reserve_of_long_rows(gpu, pages, every):
+    """Rows that are given many pages: more than a pass finds at once, spread over
+    chunks, entered between entries that hold pages."""
+    import triton_mla
+
+    rng = random.Random(pages)
+    refs = [0 if i % every == every // 2 else 1 + i % 2 for i in range(pages)]
+    free = refs.count(0)
+    counts = [1, 0, 1023, 1024, 1025, 300, 2049, 1]
+    width = max(counts) + 700
+    rows, lens, want_tokens = [], [], []
+    for c in counts:
+        c = min(c, max(free // 5 - 5, 0))
+        keep = rng.randint(0, 600)
+        row = [rng.randrange(pages) for _ in range(keep)] + [rng.choice([-1, -7, pages]) for _ in range(c)]
+        rng.shuffle(row)
+        rows.append(row + [-1] * (width - len(row)))
+        lens.append(0)
+        want_tokens.append(len(row) * 4)
+    want = ref_reserve(rows, lens, refs, want_tokens, 4)
+    assert want[2] == 0
+    got = triton_mla.reserve_pages(cuda(rows), cuda(lens), cuda(refs), cuda(want_tokens), 4)
+    assert got[0].tolist() == want[0] and got[1].tolist() == want[1] and got[2].item() == 0
+
+
 @pytest.mark.parametrize("pages", [4096, 4097, 12288, 5_000_000])
 def test_large_pools(gpu, pages):
     """Pools of several chunks: the free pages far apart, at the borders."""
