@@ -530,7 +530,8 @@ int tmla_mla_project(const void* x, int64_t x_stride, const void* w, int64_t w_s
  * Two launches (three above 256 sequences or groups or 512 blocks of rows), no
  * host synchronisation; the same inputs give the same bits. Sharing saves no
  * matrix work where a sequence's rows fill blocks of 128: tmla_mla_decode* is 8 to
- * 17% faster there, with partials rounded to dtype.
+ * 17% faster there, with partials rounded to dtype. A row that meets an infinite
+ * value within its tokens is NaN throughout, not in that dim alone.
  */
 size_t tmla_shared_workspace_bytes(int32_t batch, int32_t num_heads, int32_t num_groups, int32_t num_workers);
 int tmla_mla_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* kv,

@@ -568,3 +568,51 @@ def test_serving_run(gpu, fp8):
     again = triton_mla.mla_decode_shared(q, kv, lens, table, 320, softmax_scale=192 ** -0.5, return_lse=True,
                                          kv_scale=scale[:live.item()] if fp8 else None, share=True)
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+def test_threads_and_streams_at_once(gpu):
+    """Threads that share a stream (and so its workspace) and threads with their
+    own: page operations and decodes give what they give alone."""
+    import threading
+
+    import triton_mla
+
+    rng = random.Random(3)
+    work = []
+    for pages, batch, width in ((200, 4, 6), (20000, 30, 40), (300, 9, 8), (14000, 500, 64)):
+        rows, lens, refs = state(rng, pages, batch, width, 4)
+        rows, lens, refs, parents = cuda(rows), cuda(lens), cuda(refs), cuda([rng.randrange(batch) for _ in range(batch)])
+        kv = torch.randn(pages, 4, 576, device="cuda").bfloat16()
+        q = torch.randn(batch, 16, 576, device="cuda").bfloat16()
+        table = torch.randint(0, pages, (batch, width), device="cuda", dtype=I32)
+        common = width // 2
+        table[:, :common] = table[0, :common]
+        counts = torch.randint(4 * common, 4 * width, (batch,), device="cuda", dtype=I32)
+
+        def calls(kv=kv, q=q, rows=rows, lens=lens, refs=refs, parents=parents, table=table, counts=counts,
+                  prefix=4 * common):
+            return (*triton_mla.mla_decode_shared(q, kv, counts, table, prefix, return_lse=True, share=True),
+                    *triton_mla.reserve_pages(rows, lens, refs, 3, 4),
+                    *triton_mla.fork_sequences(kv.clone(), rows, lens, refs, parents),
+                    *triton_mla.compact_pages(kv.clone(), rows, refs))
+
+        work.append((calls, calls()))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i, stream):
+        calls, want = work[i]
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = calls()
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(i)
+
+    shared = torch.cuda.Stream()
+    threads = [threading.Thread(target=run, args=(i, shared if i < 2 else torch.cuda.Stream())) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []

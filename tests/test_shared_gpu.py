@@ -369,6 +369,29 @@ def test_values_of_one_row_far_apart(gpu):
     check(args, out, lse)
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinity_in_a_token_that_counts(gpu, sign):
+    """The rows that meet it are NaN, whichever way their scores go."""
+    args = build([3], [256], [5, 1, 70], 16)
+    args["q"][..., 100] = sign * args["q"][..., 100].abs().clamp(min=0.1)
+    args["kv_cache"][args["block_table"][1, 4].long(), 0, 100] = math.inf  # of the second sequence alone
+    out, _ = run(args)
+    assert torch.isnan(out[1]).all() and torch.isfinite(out[[0, 2]]).all()
+
+
+def test_negative_scales_of_an_fp8_cache(gpu):
+    """Pages of scales of either sign and of far exponents."""
+    import triton_mla
+
+    args = build([3], [320], [70, 1, 130], 16)
+    codes, scale = triton_mla.quantize_kv_fp8(args["kv_cache"], "page")
+    factor = torch.tensor([1.0, -1.0, 2.0 ** -9, -0.75], device="cuda")[torch.arange(scale.numel(), device="cuda") % 4]
+    scale = scale * factor.reshape(scale.shape)
+    kv = codes.view(torch.float8_e4m3fn).double() * scale.double().reshape(-1, 1, 1)
+    args["kv_cache"] = codes
+    check(args, *run(args, kv_scale=scale), kv=kv)
+
+
 def test_nan_in_a_token_that_counts(gpu):
     """A NaN that a row attends to is not lost."""
     args = build([3], [256], [5, 1, 70], 16)

@@ -109,7 +109,10 @@ def mla_decode_shared(
 
     Returns:
         out [batch, num_heads, head_dim_v] in q.dtype (and lse [batch,
-        num_heads] float32), with the q_len dim for a 4-D q.
+        num_heads] float32), with the q_len dim for a 4-D q. A head's row that
+        meets a value of infinity or NaN within its tokens is NaN throughout
+        (mla_decode: in that dim, where the score is -inf); behind them the
+        cache may hold anything.
     """
     if kv_cache.dim() == 4:
         assert kv_cache.shape[2] == 1, "MLA uses a single shared latent KV head"
